@@ -117,6 +117,72 @@ int sps_attn_bwd(int family, int B, int H, int N, int D, int dtype,
                  float sm_scale, int window, int has_pkw, int pkw,
                  void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Changes of the attention scores between their product and the softmax. For a query at position q, a
+ * key at position k and head h, with x = sm_scale * (q . k) and the distance n = max(q - k, 0):
+ *   s = softcap * tanh(x / softcap)   (x itself when softcap is 0)
+ *       - slopes[h] * n               (slopes: [H] fp32 on the device, or NULL)
+ *       + bias_table[bucket(n), h]    (bias_table: [num_buckets, H] bf16, f16 or fp32 on the device with
+ *                                      element strides table_strides, or NULL)
+ * bucket(n), with e = num_buckets / 2 (rounded down) and M = max_distance: n for n < e, else
+ * min(num_buckets - 1, e + floor((num_buckets - e) * log(n / e) / log(M / e))). 2 <= num_buckets <= 256,
+ * e < M <= 512. Entries of the table below -16384 (-inf and the types' lowest values among them) hide
+ * their pairs. softcap must be 0 or a positive finite number.
+ */
+typedef struct sps_score_change {
+  float softcap;
+  const float* slopes;
+  const void* bias_table;
+  int table_dtype;
+  int64_t table_strides[2]; /* {bucket, head} */
+  int num_buckets, max_distance;
+} sps_score_change;
+
+/* Buckets of distances 0 .. n - 1 into `out` (host memory), as the kernels take them. */
+int sps_bias_buckets(int num_buckets, int max_distance, int n, int* out);
+
+/*
+ * Document-masked causal attention (the full family) with changed scores and an optional visible
+ * prefix: query q sees key k when (k <= q or k < prefix_len[b]) and both have the same document id
+ * (docs may be NULL). prefix_len: [B] int32 or int64 on the device, unit stride, or NULL; values are
+ * clamped to [0, N]. `change` may not be NULL. Arguments and layouts otherwise as sps_attn_fwd; rows
+ * that see nothing (all their keys hidden by the table) yield 0 and lse -inf. lse receives the
+ * log2-domain log-sum-exp of the changed scores.
+ *
+ * Backward: dq, dk, dv as sps_attn_bwd; dtable: contiguous [num_buckets, H] of the table's dtype,
+ * receives the gradient of bias_table, or NULL. reuse_layout: as SPS_BWD_REUSE_LAYOUT. The result does
+ * not depend on timing (no atomics across waves). Workspace: sps_biased_workspace_bytes (num_buckets:
+ * of the table whose gradient is wanted, else 0).
+ */
+size_t sps_biased_workspace_bytes(int B, int H, int N, int has_docs, int backward, int num_buckets);
+
+int sps_biased_fwd(int B, int H, int N, int D, int dtype,
+                   const void* q, const int64_t* q_strides,
+                   const void* k, const int64_t* k_strides,
+                   const void* v, const int64_t* v_strides,
+                   void* o, const int64_t* o_strides,
+                   float* lse,
+                   const void* docs, int docs_dtype, int64_t docs_stride_b,
+                   const void* prefix_len, int prefix_dtype,
+                   float sm_scale, const sps_score_change* change,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
+int sps_biased_bwd(int B, int H, int N, int D, int dtype,
+                   const void* q, const int64_t* q_strides,
+                   const void* k, const int64_t* k_strides,
+                   const void* v, const int64_t* v_strides,
+                   const void* o, const int64_t* o_strides,
+                   const void* dout, const int64_t* dout_strides,
+                   const float* lse,
+                   void* dq, const int64_t* dq_strides,
+                   void* dk, const int64_t* dk_strides,
+                   void* dv, const int64_t* dv_strides,
+                   void* dtable,
+                   const void* docs, int docs_dtype, int64_t docs_stride_b,
+                   const void* prefix_len, int prefix_dtype,
+                   float sm_scale, const sps_score_change* change, int reuse_layout,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
 /* Passes of the backward (sps_attn_bwd runs SPS_BWD_DQ, then SPS_BWD_DKDV, on one stream). */
 #define SPS_BWD_DQ 1   /* Delta = rowsum(o * dO), and -lse, -Delta per query into the workspace, and dq
                           (reference: _attn_bwd_preprocess + _sps_bwd_dq_kernel,

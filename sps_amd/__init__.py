@@ -8,11 +8,13 @@ Drop-in replacements for the reference's attention entry points:
                       KV update in the attention's launches)
   pre-attention:      ``apply_rotary_emb``, ``rope_qkv_for_attention`` (RoPE + casts + layout, one launch)
   prefill -> decode:  ``prefill_to_decode``, ``materialize_prefill_layer_state`` (decode caches, one launch)
+  changed scores:     ``biased_attention`` (tanh cap, bias by distance, prefix; forward and backward), ``bias_buckets``
   document ids:       ``document_ids`` (EOS / left-pad rules, interleaved for the SPS families)
 All compute runs in libsps_attn.so (hand-written HIP kernels); see include/sps_attn.h.
 """
 
 from .attention import full_attention, reverse_sps_sliding_attention, sps_sliding_attention
+from .biased_attention import bias_buckets, biased_attention
 from .decode_attention import (
     KVSegment,
     masked_kv_attention,
@@ -33,6 +35,8 @@ __all__ = [
     "sps_sliding_attention",
     "reverse_sps_sliding_attention",
     "full_attention",
+    "biased_attention",
+    "bias_buckets",
     "KVSegment",
     "triton_segmented_q1_attention",
     "triton_segmented_q2_attention",

@@ -49,6 +49,10 @@ EXPORTED_SYMBOLS = (
     "sps_rope_qkv",
     "sps_prefill_to_decode",
     "sps_document_ids",
+    "sps_bias_buckets",
+    "sps_biased_workspace_bytes",
+    "sps_biased_fwd",
+    "sps_biased_bwd",
 )
 
 _i32 = C.c_int
@@ -58,6 +62,16 @@ _pi64 = C.POINTER(C.c_int64)
 _pi32 = C.POINTER(C.c_int)
 _f32 = C.c_float
 _sz = C.c_size_t
+
+
+class ScoreChange(C.Structure):
+    """sps_score_change of include/sps_attn.h."""
+
+    _fields_ = [("softcap", C.c_float), ("slopes", C.c_void_p), ("bias_table", C.c_void_p), ("table_dtype", C.c_int),
+                ("table_strides", C.c_int64 * 2), ("num_buckets", C.c_int), ("max_distance", C.c_int)]
+
+
+_pchange = C.POINTER(ScoreChange)
 
 _SIGNATURES = {
     "sps_version": (C.c_char_p, []),
@@ -148,6 +162,28 @@ _SIGNATURES = {
         + [_p],
     ),
     "sps_document_ids": (_i32, [_i32, _i32, _p, _i32, _i64, _i64, _i64, _i32, _p, _i32, _i64, _p, _p]),
+    "sps_bias_buckets": (_i32, [_i32, _i32, _i32, _pi32]),
+    "sps_biased_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "sps_biased_fwd": (
+        _i32,
+        [_i32, _i32, _i32, _i32, _i32]
+        + [_p, _pi64] * 4
+        + [_p]  # lse
+        + [_p, _i32, _i64, _p, _i32]  # docs, prefix
+        + [_f32, _pchange]
+        + [_p, _sz, _p],
+    ),
+    "sps_biased_bwd": (
+        _i32,
+        [_i32, _i32, _i32, _i32, _i32]
+        + [_p, _pi64] * 5
+        + [_p]  # lse
+        + [_p, _pi64] * 3
+        + [_p]  # dtable
+        + [_p, _i32, _i64, _p, _i32]  # docs, prefix
+        + [_f32, _pchange, _i32]
+        + [_p, _sz, _p],
+    ),
 }
 
 _lib = None

@@ -1,6 +1,6 @@
 // The dQ pass of the backward attention (see attn_bwd.hip for the two passes).
 #pragma once
-#include "attn_tiles.hpp"
+#include "attn_scores.hpp"
 
 namespace sps {
 
@@ -48,8 +48,9 @@ __device__ __forceinline__ uint16_t* wave_tile(uint16_t (&arr)[2][NG][TE], int w
   return &arr[0][0][0] + wave * TE;
 }
 
-template <int D, class E, int WAVES = dq_waves<D>()>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES, 8))) void attn_bwd_dq_kernel(const AttnArgs a) {
+template <int D, class E, int WAVES = dq_waves<D>(), class M = PlainScores>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES, 8))) void attn_bwd_dq_kernel(
+    const typename M::Args a) {
   using G = TileGeom<D>;
   constexpr int NG = dq_group<D, WAVES>();
   // Head dims of 64 and more stage K / V blocks by direct global -> LDS loads into dense swizzled
@@ -64,7 +65,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES, 8)))
   __shared__ __attribute__((aligned(16))) uint16_t sV[2][NG][TE];
   __shared__ int s_span[4 * kWaves];
 
-  const MaskSpec m = a.m;
+  MaskSpec m = a.m;
+  if constexpr (M::kOn) m.family = FAMILY_FULL;
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_index<D>();
   const int g = lane >> 5, c32 = lane & 31;
   int b, h;
@@ -76,7 +78,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES, 8)))
   const int qsafe = qvalid ? qp : 0;
   QState st;
   int run_start;
-  const bool planned = q_begin(a, tp, row, qp, s_span, st, run_start);
+  const bool planned = q_start<M>(a, tp, row, b, qp, s_span, st, run_start);
   const QPlan& plan = st.plan;
   const int nb = plan.count();
   const bool exact = row.mono;
@@ -206,6 +208,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES, 8)))
   // S * scale2 - LSE), never by rounding a scaled Q to the input type.
   const float scale2 = a.scale2, neg_lse = -lse;
   const f32x16_t c_dp = f32x16_t{} - delta;
+  const ScoreConsts consts = score_consts<M>(a, h);
+  float* lut = nullptr;
+  TableSums<M> sums;
+  if constexpr (M::kBias) {
+    lut = dynamic_lds();
+    fill_lut<true>(a, h, lut, tid, 256);
+    sums.init(a, lut + lut_len(a.far), tid, wave, lane);
+  }
 
   auto run = [&](auto exact_tag) {
     constexpr bool EXACT = decltype(exact_tag)::value;
@@ -232,17 +242,41 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES, 8)))
             sc = E::mfma(row_frag(tK, c), qf[c], sc);
             dp = E::mfma(row_frag(tV, c), dof[c], dp);
           }
+          BlockKind kind = BLOCK_FAR;
+          f32x16_t fac;  // the cap's derivative, where dS is wanted without it too
+          if constexpr (M::kOn) {
+            kind = block_kind(wave_uniform(tp.tile * kTile + wave * kBlock - t0 - 31), consts.far);
+            qs_scores<M>(sc, consts, lut, qp, t0, g, kind, neg_lse, [&](int e, float r) {
+              if constexpr (M::kCap && M::kTable)
+                fac[e] = cap_slope(r);
+              else if constexpr (M::kCap)
+                dp[e] *= cap_slope(r);
+            });
+          } else {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) sc[e] = __builtin_fmaf(sc[e], scale2, neg_lse);
+            for (int e = 0; e < 16; ++e) sc[e] = __builtin_fmaf(sc[e], scale2, neg_lse);
+          }
           if (!((full2 >> y) & 1))
             mask_partial<EXACT>(sc, lr, ws, t0, g,
                                 [&] { return qs_exact_bits<D == 128 && WAVES == 2 ? 2 : 16>(a, b, lr, plan.stream(i), t0, g, dq_doc); });
           uint32_t dsk[8];
+          if constexpr (M::kTable) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float p0 = fast_exp2(sc[2 * e]);
-            const float p1 = fast_exp2(sc[2 * e + 1]);
-            dsk[e] = E::pack2(p0 * dp[2 * e], p1 * dp[2 * e + 1]);
+            for (int e = 0; e < 16; ++e) dp[e] *= fast_exp2(sc[e]);
+            sums.add(dp, kind, qp, t0, g);
+            if constexpr (M::kCap) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) dp[e] *= fac[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dsk[e] = E::pack2(dp[2 * e], dp[2 * e + 1]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float p0 = fast_exp2(sc[2 * e]);
+              const float p1 = fast_exp2(sc[2 * e + 1]);
+              dsk[e] = E::pack2(p0 * dp[2 * e], p1 * dp[2 * e + 1]);
+            }
           }
 #pragma unroll
           for (int dc = 0; dc < G::DC; ++dc) {
@@ -264,6 +298,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES, 8)))
     run(std::true_type{});
   else
     run(std::false_type{});
+
+  if constexpr (M::kTable)
+    sums.store(a, a.dtable_part + (((int64_t)b * a.H + h) * q_tiles(m.N) + tp.tile) * a.buckets, tid, lane);
 
   uint16_t* orow = a.dq + b * a.sdq.b + h * a.sdq.h + (int64_t)qsafe * a.sdq.n;
   const float sc = a.sm_scale;

@@ -10,6 +10,7 @@
 
 #include "../../include/sps_attn.h"
 #include "attn_kernels.hpp"
+#include "attn_scores.hpp"
 #include "decode_kernels.hpp"
 
 namespace {
@@ -300,6 +301,194 @@ int sps_attn_mask(int family, int B, int N, const void* docs, int docs_dtype, in
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (docs && (rc = hip_status(sps::launch_row_layout(a, s), "document prepass"))) return rc;
   return hip_status(sps::launch_mask_dump(a, schedule, s), "mask dump");
+}
+
+}  // extern "C"
+
+namespace {
+
+// First distance of each bucket (of the next bucket that has any, where it has none), and the bucket of each distance
+// below the last bucket's first, `far`. Bucket e + j starts at the smallest n with (n / e)^m >= (M / e)^j, m = buckets
+// - e, compared by logarithms in long double: the borders that are whole numbers come out equal to within its rounding
+// (~1e-16), and over all sizes taken no other comes nearer than 1e-7.
+void distance_buckets(int buckets, int M, uint16_t* first, uint8_t* bucket, int& far) {
+  const int e = buckets / 2, m = buckets - e;
+  const long double step = std::log((long double)M / e);
+  int n = 0;
+  for (int j = 0; j < buckets; ++j) {
+    if (j < e)
+      n = j;
+    else
+      while (n < e || m * std::log((long double)n / e) < (j - e) * step - 1e-13L) ++n;
+    first[j] = (uint16_t)n;
+  }
+  far = first[buckets - 1];
+  for (int j = 0; j + 1 < buckets; ++j)
+    for (int x = first[j]; x < first[j + 1]; ++x) bucket[x] = (uint8_t)j;
+}
+
+int check_change(const sps_score_change* c) {
+  if (!c) return fail(SPS_E_INVALID, "change: null pointer");
+  if (!(std::isfinite(c->softcap) && c->softcap >= 0.f)) return fail(SPS_E_INVALID, "softcap must be 0 or a positive finite number");
+  if (!c->bias_table) return SPS_OK;
+  if (c->table_dtype != SPS_DTYPE_BF16 && c->table_dtype != SPS_DTYPE_F16 && c->table_dtype != SPS_DTYPE_F32)
+    return fail(SPS_E_UNSUPPORTED, "bias table dtype code %d not supported (bf16, f16, fp32)", c->table_dtype);
+  if (c->num_buckets < 2 || c->num_buckets > sps::kMaxBuckets)
+    return fail(SPS_E_UNSUPPORTED, "num_buckets %d not in [2, %d]", c->num_buckets, sps::kMaxBuckets);
+  if (c->max_distance <= c->num_buckets / 2 || c->max_distance > sps::kMaxDistance)
+    return fail(SPS_E_UNSUPPORTED, "max_distance %d not in (num_buckets / 2, %d]", c->max_distance, sps::kMaxDistance);
+  return SPS_OK;
+}
+
+// The score fields of the argument block from a checked change.
+void set_change(sps::BiasedArgs& a, const sps_score_change& c, float sm_scale, const void* prefix, int prefix_dtype) {
+  a.prefix = prefix;
+  a.prefix_i64 = prefix_dtype == SPS_DTYPE_I64;
+  a.cap2 = c.softcap * sps::kLog2e;
+  a.cap_in = c.softcap > 0.f ? 2.f * sps::kLog2e * sm_scale / c.softcap : 0.f;
+  a.slopes = c.slopes;
+  a.table = c.bias_table;
+  if (!c.bias_table) return;
+  a.table_dtype = c.table_dtype;
+  a.table_sj = c.table_strides[0];
+  a.table_sh = c.table_strides[1];
+  a.buckets = c.num_buckets;
+  distance_buckets(c.num_buckets, c.max_distance, a.first, a.bucket, a.far);
+}
+
+// Bytes of the query tiles' sums of the table gradient.
+size_t table_part_bytes(int B, int H, int N, int num_buckets) {
+  return align_up((size_t)B * H * sps::q_tiles(N) * num_buckets * sizeof(float));
+}
+
+int check_biased(const char* prefix_name, const void* prefix, int prefix_dtype, int D, int dtype, float sm_scale) {
+  if (prefix && prefix_dtype != SPS_DTYPE_I32 && prefix_dtype != SPS_DTYPE_I64)
+    return fail(SPS_E_INVALID, "%s must be int32 or int64 (dtype code %d)", prefix_name, prefix_dtype);
+  if (!supported_head_dim(D)) return fail(SPS_E_UNSUPPORTED, "head_dim %d not supported", D);
+  if (dtype != SPS_DTYPE_BF16 && dtype != SPS_DTYPE_F16)
+    return fail(SPS_E_UNSUPPORTED, "attention dtype code %d not supported (bf16, f16)", dtype);
+  if (!std::isfinite(sm_scale)) return fail(SPS_E_INVALID, "sm_scale must be finite");
+  return SPS_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int sps_bias_buckets(int num_buckets, int max_distance, int n, int* out) {
+  g_last_error.clear();
+  sps_score_change c = {};
+  c.bias_table = out;  // (only tested for null)
+  c.num_buckets = num_buckets;
+  c.max_distance = max_distance;
+  if (n < 0 || (n > 0 && !out)) return fail(SPS_E_INVALID, "out: null pointer or negative count");
+  if (n == 0) return SPS_OK;
+  const int rc = check_change(&c);
+  if (rc) return rc;
+  uint16_t first[sps::kMaxBuckets];
+  uint8_t bucket[sps::kMaxDistance];
+  int far;
+  distance_buckets(num_buckets, max_distance, first, bucket, far);
+  for (int i = 0; i < n; ++i) out[i] = i < far ? bucket[i] : num_buckets - 1;
+  return SPS_OK;
+}
+
+size_t sps_biased_workspace_bytes(int B, int H, int N, int has_docs, int backward, int num_buckets) {
+  if (B < 0 || H < 0 || N < 0 || num_buckets < 0) return 0;
+  return attn_layout(SPS_FAMILY_FULL, B, H, N, has_docs, backward).total +
+         (backward ? table_part_bytes(B, H, N, num_buckets) : 0);
+}
+
+int sps_biased_fwd(int B, int H, int N, int D, int dtype, const void* q, const int64_t* q_strides, const void* k,
+                   const int64_t* k_strides, const void* v, const int64_t* v_strides, void* o,
+                   const int64_t* o_strides, float* lse, const void* docs, int docs_dtype, int64_t docs_stride_b,
+                   const void* prefix_len, int prefix_dtype, float sm_scale, const sps_score_change* change,
+                   void* workspace, size_t workspace_bytes, void* stream) {
+  g_last_error.clear();
+  sps::BiasedArgs a;
+  std::memset(static_cast<void*>(&a), 0, sizeof(a));
+  int rc = setup_common(a, SPS_FAMILY_FULL, B, H, N, docs, docs_dtype, docs_stride_b, 0, 0, -1, workspace,
+                        workspace_bytes, 0);
+  if (rc || (rc = check_change(change)) || (rc = check_biased("prefix_len", prefix_len, prefix_dtype, D, dtype, sm_scale)))
+    return rc;
+  const int need = (int64_t)B * H * N > 0;
+  if ((rc = check_tensor("q", q, q_strides, need, N, D)) || (rc = check_tensor("k", k, k_strides, need, N, D)) ||
+      (rc = check_tensor("v", v, v_strides, need, N, D)) || (rc = check_tensor("o", o, o_strides, need, N, D)))
+    return rc;
+  if (need && !lse) return fail(SPS_E_INVALID, "lse: null pointer");
+  if (!need) return SPS_OK;
+  a.q = static_cast<const uint16_t*>(q);
+  a.k = static_cast<const uint16_t*>(k);
+  a.v = static_cast<const uint16_t*>(v);
+  a.out = static_cast<uint16_t*>(o);
+  a.sq = strides(q_strides);
+  a.sk = strides(k_strides);
+  a.sv = strides(v_strides);
+  a.sout = strides(o_strides);
+  a.lse = lse;
+  a.sm_scale = sm_scale;
+  a.scale2 = sm_scale * sps::kLog2e;
+  set_change(a, *change, sm_scale, prefix_len, prefix_dtype);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (docs && (rc = hip_status(sps::launch_row_layout(a, s), "document prepass"))) return rc;
+  return hip_status(sps::launch_biased_fwd(a, D, dtype == SPS_DTYPE_F16, s), "biased attention forward");
+}
+
+int sps_biased_bwd(int B, int H, int N, int D, int dtype, const void* q, const int64_t* q_strides, const void* k,
+                   const int64_t* k_strides, const void* v, const int64_t* v_strides, const void* o,
+                   const int64_t* o_strides, const void* dout, const int64_t* dout_strides, const float* lse, void* dq,
+                   const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv, const int64_t* dv_strides,
+                   void* dtable, const void* docs, int docs_dtype, int64_t docs_stride_b, const void* prefix_len,
+                   int prefix_dtype, float sm_scale, const sps_score_change* change, int reuse_layout, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+  g_last_error.clear();
+  sps::BiasedArgs a;
+  std::memset(static_cast<void*>(&a), 0, sizeof(a));
+  int rc = setup_common(a, SPS_FAMILY_FULL, B, H, N, docs, docs_dtype, docs_stride_b, 0, 0, -1, workspace,
+                        workspace_bytes, 1);
+  if (rc || (rc = check_change(change)) || (rc = check_biased("prefix_len", prefix_len, prefix_dtype, D, dtype, sm_scale)))
+    return rc;
+  const int need = (int64_t)B * H * N > 0;
+  if ((rc = check_tensor("q", q, q_strides, need, N, D)) || (rc = check_tensor("k", k, k_strides, need, N, D)) ||
+      (rc = check_tensor("v", v, v_strides, need, N, D)) || (rc = check_tensor("o", o, o_strides, need, N, D)) ||
+      (rc = check_tensor("dout", dout, dout_strides, need, N, D)) || (rc = check_tensor("dq", dq, dq_strides, need, N, D)) ||
+      (rc = check_tensor("dk", dk, dk_strides, need, N, D)) || (rc = check_tensor("dv", dv, dv_strides, need, N, D)))
+    return rc;
+  if (need && !lse) return fail(SPS_E_INVALID, "lse: null pointer");
+  if (dtable && !change->bias_table) return fail(SPS_E_INVALID, "dtable without a bias table");
+  const size_t part_at = attn_layout(SPS_FAMILY_FULL, B, H, N, docs != nullptr, 1).total;
+  const size_t total = part_at + (dtable ? table_part_bytes(B, H, N, change->num_buckets) : 0);
+  if (workspace_bytes < total) return fail(SPS_E_WORKSPACE, "workspace too small: %zu bytes < %zu", workspace_bytes, total);
+  a.q = static_cast<const uint16_t*>(q);
+  a.k = static_cast<const uint16_t*>(k);
+  a.v = static_cast<const uint16_t*>(v);
+  a.o = static_cast<const uint16_t*>(o);
+  a.dO = static_cast<const uint16_t*>(dout);
+  a.dq = static_cast<uint16_t*>(dq);
+  a.dk = static_cast<uint16_t*>(dk);
+  a.dv = static_cast<uint16_t*>(dv);
+  a.sq = strides(q_strides);
+  a.sk = strides(k_strides);
+  a.sv = strides(v_strides);
+  a.so = strides(o_strides);
+  a.sdo = strides(dout_strides);
+  a.sdq = strides(dq_strides);
+  a.sdk = strides(dk_strides);
+  a.sdv = strides(dv_strides);
+  a.lse = const_cast<float*>(lse);
+  a.sm_scale = sm_scale;
+  a.scale2 = sm_scale * sps::kLog2e;
+  set_change(a, *change, sm_scale, prefix_len, prefix_dtype);
+  if (dtable) a.dtable_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + part_at);
+  const int f16 = dtype == SPS_DTYPE_F16;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (!need) return dtable ? hip_status(sps::launch_table_gradient(a, dtable, s), "bias table gradient") : SPS_OK;
+  if (docs && !reuse_layout && (rc = hip_status(sps::launch_row_layout(a, s), "document prepass"))) return rc;
+  if ((rc = hip_status(dtable ? sps::launch_biased_dq_table(a, D, f16, s) : sps::launch_biased_dq(a, D, f16, s),
+                       "biased attention dQ")))
+    return rc;
+  if (dtable && (rc = hip_status(sps::launch_table_gradient(a, dtable, s), "bias table gradient"))) return rc;
+  return hip_status(sps::launch_biased_dkdv(a, D, f16, s), "biased attention dK/dV");
 }
 
 static int kv_bytes(int kv_dtype) { return kv_dtype == SPS_DTYPE_F32 ? 4 : 2; }
