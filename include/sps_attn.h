@@ -183,6 +183,48 @@ int sps_biased_bwd(int B, int H, int N, int D, int dtype,
                    float sm_scale, const sps_score_change* change, int reuse_layout,
                    void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Attention of T (1 .. 64) drafted tokens per sequence over up to 3 KV segments and the drafts' own
+ * ancestors, with changed scores (`change` may be NULL: unchanged). q, draft_k, draft_v: [B, T, H, D] of
+ * dtype (bf16 or f16, as the segments), strides {b, t, h}; segments as in sps_decode (strides {b, h, t},
+ * t strides not negative). parents: [B, T] int32 or int64 (unit stride along T), or NULL for a chain: -1 (a child of the cached
+ * sequence's last token) or the index of an earlier draft; a draft with any other value, or descending
+ * from such a one, is no draft: it sees nothing, no draft sees it, and its output is 0. Positions for
+ * the distances run through the segments' live keys in their order; a draft's is their number plus its
+ * depth. out: [B, T, H, D] of dtype, contiguous.
+ * Workspace: sps_tree_workspace_bytes; a workspace of that size serves every call with the same D and T, no
+ * greater B, H and scan lengths.
+ */
+size_t sps_tree_workspace_bytes(int B, int H, int D, int T, int n_seg, const int64_t* seg_scan);
+
+int sps_tree_attention(int B, int H, int D, int T, int dtype,
+                       const void* q, const int64_t* q_strides, int n_seg,
+                       const void* const* seg_k, const int64_t* seg_k_strides,
+                       const void* const* seg_v, const int64_t* seg_v_strides,
+                       const void* const* seg_len, const int* seg_len_dtype, const int* seg_len_per_head,
+                       const int64_t* seg_scan,
+                       const void* draft_k, const int64_t* draft_k_strides,
+                       const void* draft_v, const int64_t* draft_v_strides,
+                       const void* parents, int parents_dtype, int64_t parents_stride_b,
+                       float sm_scale, const sps_score_change* change, void* out,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Appends the accepted drafts of each sequence to its cache: the path from a root to draft last[b]
+ * (parents as in sps_tree_attention; last: [B] int32 or int64) goes to rows len .. of k and v
+ * [B, H, storage, D], and the length advances. Rows past the storage are dropped, and the length stops there; nothing happens where last[b]
+ * is no draft or a length is negative or at the storage. Lengths: [B, H] (strides {b, h}) or, with
+ * len_per_head 0, [B]. dtype (bf16, f16 or fp32) is that of the cache and the drafts alike; strides are
+ * {k: b, h, t, v: b, h, t} for the cache and {b, t, h} for the drafts. The caches may not overlap the drafts.
+ */
+int sps_commit_drafts(int B, int H, int D, int T, int dtype,
+                      void* k, void* v, const int64_t* kv_strides, int storage,
+                      void* len, int len_dtype, int len_per_head, const int64_t* len_strides,
+                      const void* draft_k, const int64_t* draft_k_strides,
+                      const void* draft_v, const int64_t* draft_v_strides,
+                      const void* parents, int parents_dtype, int64_t parents_stride_b,
+                      const void* last, int last_dtype, void* stream);
+
 /* Passes of the backward (sps_attn_bwd runs SPS_BWD_DQ, then SPS_BWD_DKDV, on one stream). */
 #define SPS_BWD_DQ 1   /* Delta = rowsum(o * dO), and -lse, -Delta per query into the workspace, and dq
                           (reference: _attn_bwd_preprocess + _sps_bwd_dq_kernel,

@@ -9,6 +9,7 @@ Drop-in replacements for the reference's attention entry points:
   pre-attention:      ``apply_rotary_emb``, ``rope_qkv_for_attention`` (RoPE + casts + layout, one launch)
   prefill -> decode:  ``prefill_to_decode``, ``materialize_prefill_layer_state`` (decode caches, one launch)
   changed scores:     ``biased_attention`` (tanh cap, bias by distance, prefix; forward and backward), ``bias_buckets``
+  drafted tokens:     ``tree_attention`` (a tree, a chain or one token over the caches), ``commit_drafts``
   document ids:       ``document_ids`` (EOS / left-pad rules, interleaved for the SPS families)
 All compute runs in libsps_attn.so (hand-written HIP kernels); see include/sps_attn.h.
 """
@@ -29,6 +30,7 @@ from .decode_attention_fast import (
 from .doc_ids import document_ids, left_padded_document_ids
 from .integration import install_into_modeling
 from .rope import apply_rotary_emb, rope_qkv_for_attention
+from .tree_attention import commit_drafts, tree_attention
 from .prefill_state import materialize_prefill_layer_state, prefill_to_decode
 
 __all__ = [
@@ -44,6 +46,8 @@ __all__ = [
     "fused_sps_kv_update",
     "segmented_q1_attention_with_kv_update",
     "segmented_q2_attention_with_kv_update",
+    "tree_attention",
+    "commit_drafts",
     "document_ids",
     "left_padded_document_ids",
     "install_into_modeling",

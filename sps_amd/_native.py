@@ -53,6 +53,9 @@ EXPORTED_SYMBOLS = (
     "sps_biased_workspace_bytes",
     "sps_biased_fwd",
     "sps_biased_bwd",
+    "sps_tree_workspace_bytes",
+    "sps_tree_attention",
+    "sps_commit_drafts",
 )
 
 _i32 = C.c_int
@@ -183,6 +186,22 @@ _SIGNATURES = {
         + [_p, _i32, _i64, _p, _i32]  # docs, prefix
         + [_f32, _pchange, _i32]
         + [_p, _sz, _p],
+    ),
+    "sps_tree_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _pi64]),
+    "sps_tree_attention": (
+        _i32,
+        [_i32] * 5
+        + [_p, _pi64, _i32]
+        + [C.POINTER(_p), _pi64, C.POINTER(_p), _pi64, C.POINTER(_p), _pi32, _pi32, _pi64]
+        + [_p, _pi64, _p, _pi64, _p, _i32, _i64]  # drafts, parents
+        + [_f32, _pchange, _p]
+        + [_p, _sz, _p],
+    ),
+    "sps_commit_drafts": (
+        _i32,
+        [_i32] * 5
+        + [_p, _p, _pi64, _i32, _p, _i32, _i32, _pi64]  # cache, lengths
+        + [_p, _pi64, _p, _pi64, _p, _i32, _i64, _p, _i32, _p],  # drafts, parents, last
     ),
 }
 

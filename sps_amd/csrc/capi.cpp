@@ -12,6 +12,7 @@
 #include "attn_kernels.hpp"
 #include "attn_scores.hpp"
 #include "decode_kernels.hpp"
+#include "tree_kernels.hpp"
 
 namespace {
 
@@ -489,6 +490,210 @@ int sps_biased_bwd(int B, int H, int N, int D, int dtype, const void* q, const i
     return rc;
   if (dtable && (rc = hip_status(sps::launch_table_gradient(a, dtable, s), "bias table gradient"))) return rc;
   return hip_status(sps::launch_biased_dkdv(a, D, f16, s), "biased attention dK/dV");
+}
+
+}  // extern "C"
+
+namespace {
+
+int check_index_dtype(const char* name, const void* p, int dtype) {
+  if (p && dtype != SPS_DTYPE_I32 && dtype != SPS_DTYPE_I64)
+    return fail(SPS_E_INVALID, "%s must be int32 or int64 (dtype code %d)", name, dtype);
+  return SPS_OK;
+}
+
+// Rows of a [B, T, H, D] tensor (strides b, t, h, of `bytes`-sized elements): 16-byte aligned.
+int check_rows(const char* name, const void* p, const int64_t* st, int bytes) {
+  if (!p || !st) return fail(SPS_E_INVALID, "%s: null pointer", name);
+  if (!aligned16(p)) return fail(SPS_E_INVALID, "%s: base pointer must be 16-byte aligned", name);
+  for (int i = 0; i < 3; ++i)
+    if (st[i] * bytes % 16 != 0) return fail(SPS_E_INVALID, "%s: strides must be multiples of 16 bytes", name);
+  return SPS_OK;
+}
+
+int check_drafts(int B, int H, int D, int T) {
+  if (B < 0 || H < 0) return fail(SPS_E_INVALID, "negative size B=%d H=%d", B, H);
+  if (B > 65535 || H > 65535) return fail(SPS_E_UNSUPPORTED, "B=%d or H=%d above 65535", B, H);
+  if (T < 1 || T > sps::kMaxDrafts) return fail(SPS_E_UNSUPPORTED, "%d drafts: 1 to %d are taken", T, sps::kMaxDrafts);
+  if (!supported_head_dim(D)) return fail(SPS_E_UNSUPPORTED, "head_dim %d not supported", D);
+  return SPS_OK;
+}
+
+int64_t tree_chunks(int n_seg, const int64_t* scan, int chunk) {
+  int64_t n = 0;
+  for (int s = 0; s < n_seg; ++s) n += (scan[s] + chunk - 1) / chunk;
+  return n;
+}
+
+size_t tree_part_bytes(int B, int H, int D, int T, int64_t chunks) {
+  return align_up((size_t)B * H * (chunks + 1) * T * sps::tree_record_floats(D) * sizeof(float));
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t sps_tree_workspace_bytes(int B, int H, int D, int T, int n_seg, const int64_t* seg_scan) {
+  if (B < 0 || H < 0 || T < 1 || T > sps::kMaxDrafts || !supported_head_dim(D) || n_seg < 0 ||
+      n_seg > sps::kMaxDecodeSegs)
+    return 0;
+  for (int s = 0; s < n_seg; ++s)
+    if (seg_scan[s] < 0) return 0;
+  const int chunk = sps::tree_chunk_keys(B, H, D, T, n_seg, seg_scan);
+  return tree_part_bytes(B, H, D, T, tree_chunks(n_seg, seg_scan, chunk));
+}
+
+int sps_tree_attention(int B, int H, int D, int T, int dtype, const void* q, const int64_t* q_strides, int n_seg,
+                       const void* const* seg_k, const int64_t* seg_k_strides, const void* const* seg_v,
+                       const int64_t* seg_v_strides, const void* const* seg_len, const int* seg_len_dtype,
+                       const int* seg_len_per_head, const int64_t* seg_scan, const void* draft_k,
+                       const int64_t* draft_k_strides, const void* draft_v, const int64_t* draft_v_strides,
+                       const void* parents, int parents_dtype, int64_t parents_stride_b, float sm_scale,
+                       const sps_score_change* change, void* out, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  g_last_error.clear();
+  int rc = check_drafts(B, H, D, T);
+  if (rc) return rc;
+  if (dtype != SPS_DTYPE_BF16 && dtype != SPS_DTYPE_F16)
+    return fail(SPS_E_UNSUPPORTED, "tree attention dtype code %d not supported (bf16, f16)", dtype);
+  if (!std::isfinite(sm_scale)) return fail(SPS_E_INVALID, "sm_scale must be finite");
+  if (n_seg < 0 || n_seg > sps::kMaxDecodeSegs)
+    return fail(SPS_E_INVALID, "at most %d segments (got %d)", sps::kMaxDecodeSegs, n_seg);
+  const sps_score_change none = {};
+  if (!change) change = &none;
+  if ((rc = check_change(change)) || (rc = check_index_dtype("parents", parents, parents_dtype))) return rc;
+  if ((int64_t)B * H == 0) return SPS_OK;
+  if ((rc = check_rows("q", q, q_strides, 2)) || (rc = check_rows("draft_k", draft_k, draft_k_strides, 2)) ||
+      (rc = check_rows("draft_v", draft_v, draft_v_strides, 2)))
+    return rc;
+  if (draft_k_strides[1] < 0 || draft_v_strides[1] < 0) return fail(SPS_E_INVALID, "drafts: negative stride");
+  if (!out) return fail(SPS_E_INVALID, "out: null pointer");
+  int64_t keys = 0;
+  for (int s = 0; s < n_seg; ++s) {
+    if (seg_scan[s] < 0) return fail(SPS_E_INVALID, "segment %d: scan length %lld out of range", s, (long long)seg_scan[s]);
+    keys += seg_scan[s];
+    if (keys > (1 << 30)) return fail(SPS_E_UNSUPPORTED, "the segments' scan lengths exceed 2^30 keys");
+  }
+  sps::TreeArgs a;
+  std::memset(static_cast<void*>(&a), 0, sizeof(a));
+  // A workspace for larger sizes may be too small for this call's own, shorter chunks: longer ones serve then.
+  int chunk = sps::tree_chunk_keys(B, H, D, T, n_seg, seg_scan);
+  while (workspace_bytes < tree_part_bytes(B, H, D, T, tree_chunks(n_seg, seg_scan, chunk)) && chunk < 4096) chunk *= 2;
+  const int64_t chunks = tree_chunks(n_seg, seg_scan, chunk);
+  const size_t need = tree_part_bytes(B, H, D, T, chunks);
+  if (workspace_bytes < need) return fail(SPS_E_WORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, need);
+  if (!workspace) return fail(SPS_E_INVALID, "workspace: null pointer");
+  a.B = B;
+  a.H = H;
+  a.T = T;
+  a.n_seg = n_seg;
+  int base = 0;
+  const int64_t most = (int64_t)INT32_MAX / 2 - 1024;  // bytes of a chunk's rows: 32-bit offsets
+  for (int s = 0; s < n_seg; ++s) {
+    sps::TreeSeg& sg = a.seg[s];
+    sg.scan = (int)seg_scan[s];
+    sg.chunk_base = base;
+    base += (sg.scan + chunk - 1) / chunk;
+    if (sg.scan == 0) continue;
+    if (!seg_len[s]) return fail(SPS_E_INVALID, "segment %d: null pointer", s);
+    const int64_t *ks = seg_k_strides + 3 * s, *vs = seg_v_strides + 3 * s;
+    if ((rc = check_rows("segment keys", seg_k[s], ks, 2)) || (rc = check_rows("segment values", seg_v[s], vs, 2)) ||
+        (rc = check_index_dtype("segment lengths", seg_len[s], seg_len_dtype[s])))
+      return rc;
+    if (ks[2] < 0 || vs[2] < 0) return fail(SPS_E_INVALID, "segment %d: negative key stride", s);
+    if (ks[2] * chunk > most || vs[2] * chunk > most)
+      return fail(SPS_E_UNSUPPORTED, "segment %d: key stride too large", s);
+    sg.k = static_cast<const uint16_t*>(seg_k[s]);
+    sg.v = static_cast<const uint16_t*>(seg_v[s]);
+    sg.ksb = ks[0];
+    sg.ksh = ks[1];
+    sg.kst = ks[2];
+    sg.vsb = vs[0];
+    sg.vsh = vs[1];
+    sg.vst = vs[2];
+    sg.len = seg_len[s];
+    sg.len_i64 = seg_len_dtype[s] == SPS_DTYPE_I64;
+    sg.len_per_head = seg_len_per_head[s] != 0;
+  }
+  if (draft_k_strides[1] * T > most || draft_v_strides[1] * T > most)
+    return fail(SPS_E_UNSUPPORTED, "drafts: stride too large");
+  auto btH = [](const int64_t* st) { return sps::Strides3{st[0], st[2], st[1]}; };  // {b, h, draft}
+  a.q = static_cast<const uint16_t*>(q);
+  a.dk = static_cast<const uint16_t*>(draft_k);
+  a.dv = static_cast<const uint16_t*>(draft_v);
+  a.sq = btH(q_strides);
+  a.sdk = btH(draft_k_strides);
+  a.sdv = btH(draft_v_strides);
+  a.parents = parents;
+  a.parents_i64 = parents_dtype == SPS_DTYPE_I64;
+  a.parents_sb = parents_stride_b;
+  a.part = static_cast<float*>(workspace);
+  a.n_chunks = (int)chunks;
+  a.chunk_keys = chunk;
+  a.out = static_cast<uint16_t*>(out);
+  a.cap = change->softcap > 0.f;
+  a.bias = change->slopes || change->bias_table;
+  a.s.scale2 = sm_scale * sps::kLog2e;
+  set_change(a.s, *change, sm_scale, nullptr, 0);
+  return hip_status(sps::launch_tree(a, D, dtype == SPS_DTYPE_F16, static_cast<hipStream_t>(stream)), "tree attention");
+}
+
+int sps_commit_drafts(int B, int H, int D, int T, int dtype, void* k, void* v, const int64_t* kv_strides, int storage,
+                      void* len, int len_dtype, int len_per_head, const int64_t* len_strides, const void* draft_k,
+                      const int64_t* draft_k_strides, const void* draft_v, const int64_t* draft_v_strides,
+                      const void* parents, int parents_dtype, int64_t parents_stride_b, const void* last,
+                      int last_dtype, void* stream) {
+  g_last_error.clear();
+  int rc = check_drafts(B, H, D, T);
+  if (rc) return rc;
+  if (dtype != SPS_DTYPE_BF16 && dtype != SPS_DTYPE_F16 && dtype != SPS_DTYPE_F32)
+    return fail(SPS_E_UNSUPPORTED, "cache dtype code %d not supported", dtype);
+  if (storage < 0) return fail(SPS_E_INVALID, "negative storage %d", storage);
+  if ((rc = check_index_dtype("parents", parents, parents_dtype)) || (rc = check_index_dtype("lengths", len, len_dtype)) ||
+      (rc = check_index_dtype("last", last, last_dtype)))
+    return rc;
+  if ((int64_t)B * H == 0 || storage == 0) return SPS_OK;
+  const int bytes = dtype == SPS_DTYPE_F32 ? 4 : 2;
+  if (!kv_strides || !len_strides) return fail(SPS_E_INVALID, "strides: null pointer");
+  if ((rc = check_rows("k", k, kv_strides, bytes)) || (rc = check_rows("v", v, kv_strides + 3, bytes)) ||
+      (rc = check_rows("draft_k", draft_k, draft_k_strides, bytes)) ||
+      (rc = check_rows("draft_v", draft_v, draft_v_strides, bytes)))
+    return rc;
+  if (!len || !last) return fail(SPS_E_INVALID, "lengths or last: null pointer");
+  sps::CommitArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.B = B;
+  a.H = H;
+  a.T = T;
+  a.row_bytes = D * bytes;
+  a.k = static_cast<char*>(k);
+  a.v = static_cast<char*>(v);
+  a.ksb = kv_strides[0] * bytes;
+  a.ksh = kv_strides[1] * bytes;
+  a.kst = kv_strides[2] * bytes;
+  a.vsb = kv_strides[3] * bytes;
+  a.vsh = kv_strides[4] * bytes;
+  a.vst = kv_strides[5] * bytes;
+  a.storage = storage;
+  a.len = len;
+  a.len_i64 = len_dtype == SPS_DTYPE_I64;
+  a.len_per_head = len_per_head != 0;
+  a.len_sb = len_strides[0];
+  a.len_sh = len_per_head ? len_strides[1] : 0;
+  a.dk = static_cast<const char*>(draft_k);
+  a.dv = static_cast<const char*>(draft_v);
+  a.dk_sb = draft_k_strides[0] * bytes;
+  a.dk_st = draft_k_strides[1] * bytes;
+  a.dk_sh = draft_k_strides[2] * bytes;
+  a.dv_sb = draft_v_strides[0] * bytes;
+  a.dv_st = draft_v_strides[1] * bytes;
+  a.dv_sh = draft_v_strides[2] * bytes;
+  a.parents = parents;
+  a.parents_i64 = parents_dtype == SPS_DTYPE_I64;
+  a.parents_sb = parents_stride_b;
+  a.last = last;
+  a.last_i64 = last_dtype == SPS_DTYPE_I64;
+  return hip_status(sps::launch_commit(a, static_cast<hipStream_t>(stream)), "draft commit");
 }
 
 static int kv_bytes(int kv_dtype) { return kv_dtype == SPS_DTYPE_F32 ? 4 : 2; }
