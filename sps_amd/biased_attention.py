@@ -204,6 +204,12 @@ def biased_attention(
     positions of each row (pads included) that every query of the row sees, later ones too, within its document; a
     key ahead of its query has distance 0. Queries that see no key yield 0. As in ``full_attention``, a non-finite value row can reach
     the outputs of other queries of its 32-query tile, whose weight of it is 0."""
+    if not torch.compiler.is_compiling():
+        # Ordinary eager calls run in native code from here on; None: the general path below.
+        o = N.binding().biased_attention(q, k, v, sm_scale, softcap, slopes, bias_table, max_distance, documents_idx_BxT,
+                                         prefix_len_B)
+        if o is not None:
+            return o
     _validate(q, k, v, N.FAMILY_FULL, documents_idx_BxT)
     cap = check_change(softcap, slopes, bias_table, max_distance, q.shape[1], q.device)
     if k.device != q.device or v.device != q.device:

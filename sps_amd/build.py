@@ -54,8 +54,8 @@ SOURCE_FLAGS = {
     "attn_bwd.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "attn_bwd_split.hip": ["-mllvm", "-amdgpu-use-amdgpu-trackers=1"],
     "attn_biased_fwd.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
-    "attn_biased_dq.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
-    "attn_biased_dq_table.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
+    "attn_biased_dq.hip": ["-mllvm", "-amdgpu-use-amdgpu-trackers=1"],
+    "attn_biased_dq_table.hip": ["-mllvm", "-amdgpu-use-amdgpu-trackers=1"],
     "attn_biased_dkdv.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "attn_biased_split.hip": ["-mllvm", "-amdgpu-use-amdgpu-trackers=1"],
 }

@@ -10,10 +10,10 @@ static hipError_t launch_m(const BiasedArgs& a, hipStream_t stream) {
   if (nq == 0) return hipSuccess;
   const size_t lds = M::kBias ? lut_len(a.far) * sizeof(float) * (M::kTable ? 1 + kTableCopies : 1) : 0;
   const dim3 grid((unsigned)nq), block(256);
-  if (D == 128 && dq_two_waves(a.m, nq))
-    hipLaunchKernelGGL((attn_bwd_dq_kernel<D, E, D == 128 ? 2 : dq_waves<D>(), M>), grid, block, lds, stream, a);
+  if (D == 128 && dq_two_waves_changed(nq))
+    hipLaunchKernelGGL((attn_bwd_dq_kernel<D, E, D == 128 ? 2 : dq_waves_changed<D, M>(), M>), grid, block, lds, stream, a);
   else
-    hipLaunchKernelGGL((attn_bwd_dq_kernel<D, E, dq_waves<D>(), M>), grid, block, lds, stream, a);
+    hipLaunchKernelGGL((attn_bwd_dq_kernel<D, E, dq_waves_changed<D, M>(), M>), grid, block, lds, stream, a);
   return hipGetLastError();
 }
 

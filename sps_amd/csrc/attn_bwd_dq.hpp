@@ -29,6 +29,16 @@ constexpr int bwd_waves() { return D <= 64 ? 2 : 1; }
 // 227 / 190 / 191).
 template <int D>
 constexpr int dq_waves() { return D == 64 ? 3 : bwd_waves<D>(); }
+// With changed scores at D = 64, two waves where the scores are capped or the table's gradient is summed: at three those
+// spill up to 109 VGPRs inside the loop, whose reloads wait for the direct loads before them.
+template <int D, class M>
+constexpr int dq_waves_changed() { return D == 64 && (M::kCap || M::kTable) ? 2 : dq_waves<D>(); }
+
+// With changed scores the two-wave form at D = 128 is built under the default scheduler with the register trackers and
+// the register-lean swizzle, which leaves it at most 13 spilled VGPRs (69 to 135 under ILP with the other: capped,
+// B2 H16 N2048, 156 -> 97 us), and it is taken wherever tiles share a CU (360 tiles of packed documents, capped and
+// biased, 67 against 76 us in the one-wave form).
+inline bool dq_two_waves_changed(int64_t tiles) { return tiles > 256; }
 template <int D, int WAVES>
 constexpr int dq_group() { return D == 64 || (D == 128 && WAVES == 2) ? 2 : bwd_group<D>(); }
 
@@ -59,7 +69,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES, 8)))
   constexpr bool kDma = D >= 64;
   // The conflict-free swizzle costs a few address VGPRs: at D = 64 (3 waves per SIMD) and D = 256
   // they would spill, so those keep the register-lean one.
-  using DT = DmaTile<kDma ? D : 64, D == 128>;
+  using DT = DmaTile<kDma ? D : 64, D == 128 && !M::kOn>;
   constexpr int TE = kDma ? DT::ELEMS : G::ELEMS;
   __shared__ __attribute__((aligned(16))) uint16_t sK[2][NG][TE];  // [buffer][block of the group]
   __shared__ __attribute__((aligned(16))) uint16_t sV[2][NG][TE];
@@ -214,7 +224,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES, 8)))
   if constexpr (M::kBias) {
     lut = dynamic_lds();
     fill_lut<true>(a, h, lut, tid, 256);
-    sums.init(a, lut + lut_len(a.far), tid, wave, lane);
+    sums.init(a, lut + lut_len(a.far), tid, wave);
   }
 
   auto run = [&](auto exact_tag) {
@@ -263,7 +273,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES, 8)))
           if constexpr (M::kTable) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) dp[e] *= fast_exp2(sc[e]);
-            sums.add(dp, kind, qp, t0, g);
+            sums.add(dp, kind, tp.tile * kTile + wave * kBlock, t0, lane);
             if constexpr (M::kCap) {
 #pragma unroll
               for (int e = 0; e < 16; ++e) dp[e] *= fac[e];

@@ -276,6 +276,366 @@ py::object attention(py::handle q_, py::handle k_, py::handle v_, py::handle sca
 }
 
 // ---------------------------------------------------------------------------------------------
+// Attention with changed scores, draft trees.
+// ---------------------------------------------------------------------------------------------
+// The score change of a call from Python arguments (softcap, slopes, bias_table, max_distance) for h heads on
+// `device`; false: not a call for this path.
+struct Change {
+  Tensor slopes, table;
+  double softcap = 0.0;
+  int max_distance = 0;
+  int buckets() const { return table.defined() ? (int)table.size(0) : 0; }
+  sps_score_change args() const {
+    sps_score_change c = {};
+    c.softcap = (float)softcap;
+    if (slopes.defined()) c.slopes = slopes.data_ptr<float>();
+    if (table.defined()) {
+      c.bias_table = table.data_ptr();
+      c.table_dtype = float_code(table.scalar_type());
+      c.table_strides[0] = table.stride(0);
+      c.table_strides[1] = table.stride(1);
+      c.num_buckets = buckets();
+      c.max_distance = max_distance;
+    }
+    return c;
+  }
+};
+
+bool fit_change(const Change& c, int64_t h, c10::Device device) {
+  if (c.slopes.defined() && (c.slopes.scalar_type() != at::kFloat || c.slopes.dim() != 1 || c.slopes.size(0) != h ||
+                             !c.slopes.is_contiguous() || c.slopes.device() != device))
+    return false;
+  if (c.table.defined() &&
+      (float_code(c.table.scalar_type()) < 0 || c.table.dim() != 2 || c.table.size(1) != h ||
+       c.table.device() != device || c.table.size(0) < 2 || c.table.size(0) > 256 ||
+       c.max_distance <= c.table.size(0) / 2 || c.max_distance > 512))
+    return false;
+  return true;
+}
+
+bool read_change(py::handle softcap, py::handle slopes, py::handle table, py::handle max_distance, int64_t h,
+                 c10::Device device, Change& c) {
+  if (!softcap.is_none()) {
+    if (!(PyFloat_CheckExact(softcap.ptr()) || PyLong_CheckExact(softcap.ptr()))) return false;
+    c.softcap = PyFloat_AsDouble(softcap.ptr());
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      return false;
+    }
+    if (!std::isfinite((float)c.softcap) || !((float)c.softcap > 0.f)) return false;
+  }
+  if (!slopes.is_none()) {
+    c.slopes = plain(slopes);
+    if (!c.slopes.defined()) return false;
+  }
+  if (!table.is_none()) {
+    c.table = plain(table);
+    const auto top = as_int(max_distance);
+    if (!c.table.defined() || !top) return false;
+    c.max_distance = *top;
+  }
+  return fit_change(c, h, device);
+}
+
+std::optional<Tensor> optional(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+
+AttnOut biased_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& docs, const Tensor& prefix,
+                       const Change& c, double sm_scale, int backward_buckets) {
+  RECORD_FUNCTION("sps_amd::biased_attention_fwd", std::vector<c10::IValue>());
+  c10::DeviceGuard on_device(q.device());
+  const auto s = q.sizes();
+  const int b = (int)s[0], h = (int)s[1], n = (int)s[2], d = (int)s[3];
+  AttnOut r;
+  r.o = at::empty({b, n, h, d}, q.options()).transpose(1, 2);
+  r.lse = at::empty({b, h, n}, q.options().dtype(at::kFloat));
+  const bool has_docs = docs.defined(), keep = has_docs && backward_buckets >= 0;
+  const size_t bytes = sps_biased_workspace_bytes(b, h, n, has_docs, keep, std::max(backward_buckets, 0));
+  if (bytes) r.ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+  const sps_score_change change = c.args();
+  check("sps_biased_fwd",
+        sps_biased_fwd(b, h, n, d, float_code(q.scalar_type()), q.data_ptr(), q.strides().data(), k.data_ptr(),
+                       k.strides().data(), v.data_ptr(), v.strides().data(), r.o.data_ptr(), r.o.strides().data(),
+                       r.lse.data_ptr<float>(), has_docs ? docs.data_ptr() : nullptr,
+                       has_docs ? index_code(docs.scalar_type()) : 0, has_docs ? docs.stride(0) : 0,
+                       prefix.defined() ? prefix.data_ptr() : nullptr,
+                       prefix.defined() ? index_code(prefix.scalar_type()) : SPS_DTYPE_I32, (float)sm_scale, &change,
+                       bytes ? r.ws.data_ptr() : nullptr, bytes, stream_of(q)));
+  return r;
+}
+
+struct BiasedFunction : torch::autograd::Function<BiasedFunction> {
+  static constexpr bool is_traceable = true;  // as AttentionFunction's
+
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                        const std::optional<Tensor>& table, const std::optional<Tensor>& docs_opt,
+                        const std::optional<Tensor>& prefix_opt, const std::optional<Tensor>& slopes, double sm_scale,
+                        double softcap, int64_t max_distance, int64_t backward_buckets) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor docs = docs_opt.value_or(Tensor()), prefix = prefix_opt.value_or(Tensor());
+    const Change c{slopes.value_or(Tensor()), table.value_or(Tensor()), softcap, (int)max_distance};
+    AttnOut r = biased_forward(q, k, v, docs, prefix, c, sm_scale, (int)backward_buckets);
+    if (!docs.defined()) r.ws = Tensor();
+    ctx->save_for_backward({q, k, v, r.o, r.lse, docs, prefix, c.slopes, c.table, r.ws});
+    ctx->saved_data["scales"] = std::vector<double>{sm_scale, softcap};
+    ctx->saved_data["table"] = std::vector<int64_t>{max_distance, backward_buckets};
+    return r.o;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &lse = saved[4], &docs = saved[5],
+                 &prefix = saved[6];
+    Tensor ws = saved[9];
+    const auto scales = ctx->saved_data["scales"].toDoubleVector();
+    const auto sizes = ctx->saved_data["table"].toIntVector();
+    const Change c{saved[7], saved[8], scales[1], (int)sizes[0]};
+    const int64_t buckets = sizes[1];
+    Tensor dout = grads[0];
+    if (!dout.defined()) dout = at::zeros_like(o);
+    bool native = !at::GradMode::is_enabled() && plain_thread() && lse.is_contiguous();
+    for (const Tensor* t : std::initializer_list<const Tensor*>{&q, &k, &v, &o, &dout})
+      native = native && plain_tensor(*t) && t->scalar_type() == q.scalar_type() && t->device() == q.device();
+    for (const Tensor* t : std::initializer_list<const Tensor*>{&lse, &docs, &prefix, &c.slopes, &ws})
+      native = native && (!t->defined() || (plain_tensor(*t) && t->is_contiguous() && t->device() == q.device()));
+    native = native && (!c.table.defined() || plain_tensor(c.table)) && fit_change(c, q.size(1), q.device());
+    for (const Tensor* t : {&q, &k, &v, &o}) native = native && attn_readable(*t) && dense(*t);
+    if (!native) {
+      static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("sps_amd::biased_attention_bwd", "");
+      auto maybe = [](const Tensor& t) { return t.defined() ? c10::IValue(t) : c10::IValue(); };
+      std::vector<c10::IValue> stack{
+          dout, q, k, v, o, lse, maybe(docs), maybe(prefix), maybe(c.slopes), maybe(c.table),
+          ws.defined() ? ws : at::empty({0}, q.options().dtype(at::kByte)), scales[0], scales[1], sizes[0], buckets};
+      op.callBoxed(&stack);
+      return {stack[0].toTensor(), stack[1].toTensor(), stack[2].toTensor(), buckets ? stack[3].toTensor() : Tensor(),
+              {}, {}, {}, {}, {}, {}, {}};
+    }
+    RECORD_FUNCTION("sps_amd::biased_attention_bwd", std::vector<c10::IValue>());
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::DeviceGuard on_device(q.device());
+    if (!attn_readable(dout)) dout = dout.contiguous();
+    const auto s = q.sizes();
+    const int b = (int)s[0], h = (int)s[1], n = (int)s[2], d = (int)s[3];
+    const bool has_docs = docs.defined(), reuse = has_docs && ws.defined();
+    const Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
+    Tensor dtable;
+    if (buckets) dtable = at::empty({buckets, h}, c.table.options());
+    if (!reuse)
+      ws = at::empty({(int64_t)sps_biased_workspace_bytes(b, h, n, has_docs, 1, (int)buckets)}, q.options().dtype(at::kByte));
+    const sps_score_change change = c.args();
+    check("sps_biased_bwd",
+          sps_biased_bwd(b, h, n, d, float_code(q.scalar_type()), q.data_ptr(), q.strides().data(), k.data_ptr(),
+                         k.strides().data(), v.data_ptr(), v.strides().data(), o.data_ptr(), o.strides().data(),
+                         dout.data_ptr(), dout.strides().data(), lse.data_ptr<float>(), dq.data_ptr(),
+                         dq.strides().data(), dk.data_ptr(), dk.strides().data(), dv.data_ptr(), dv.strides().data(),
+                         buckets ? dtable.data_ptr() : nullptr, has_docs ? docs.data_ptr() : nullptr,
+                         has_docs ? index_code(docs.scalar_type()) : 0, has_docs ? docs.stride(0) : 0,
+                         prefix.defined() ? prefix.data_ptr() : nullptr,
+                         prefix.defined() ? index_code(prefix.scalar_type()) : SPS_DTYPE_I32, (float)scales[0], &change,
+                         reuse, ws.data_ptr(), (size_t)ws.numel(), stream_of(q)));
+    return {dq, dk, dv, dtable, {}, {}, {}, {}, {}, {}, {}};
+  }
+};
+
+py::object biased_attention(py::handle q_, py::handle k_, py::handle v_, py::handle scale_, py::handle softcap_,
+                            py::handle slopes_, py::handle table_, py::handle max_distance_, py::handle docs_,
+                            py::handle prefix_) {
+  if (!plain_thread() || !(PyFloat_CheckExact(scale_.ptr()) || PyLong_CheckExact(scale_.ptr()))) return py::none();
+  const double sm_scale = PyFloat_AsDouble(scale_.ptr());
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return py::none();
+  }
+  const Tensor q = plain(q_), k = plain(k_), v = plain(v_);
+  if (!q.defined() || !k.defined() || !v.defined() || !std::isfinite((float)sm_scale)) return py::none();
+  const auto type = q.scalar_type();
+  if ((type != at::kBFloat16 && type != at::kHalf) || k.scalar_type() != type || v.scalar_type() != type ||
+      q.dim() != 4 || k.sizes() != q.sizes() || v.sizes() != q.sizes() || k.device() != q.device() ||
+      v.device() != q.device() || q.numel() == 0 || !decode_head_dim(q.size(3)))
+    return py::none();
+  const int64_t n = q.size(2);
+  if (!fits_int(q.size(0)) || !fits_int(q.size(1)) || !fits_int(n) || !attn_readable(q) || !attn_readable(k) ||
+      !attn_readable(v))
+    return py::none();
+  Tensor docs, prefix;
+  if (!docs_.is_none()) {
+    docs = plain(docs_);
+    if (!docs.defined() || docs.dim() != 2 || docs.size(0) != q.size(0) || docs.size(1) != n ||
+        index_code(docs.scalar_type()) < 0 || docs.device() != q.device() || !docs.is_contiguous())
+      return py::none();
+  }
+  if (!prefix_.is_none()) {
+    prefix = plain(prefix_);
+    if (!prefix.defined() || prefix.dim() != 1 || prefix.size(0) != q.size(0) ||
+        index_code(prefix.scalar_type()) < 0 || prefix.device() != q.device() || !prefix.is_contiguous())
+      return py::none();
+  }
+  Change c;
+  if (!read_change(softcap_, slopes_, table_, max_distance_, q.size(1), q.device(), c)) return py::none();
+  if (c.slopes.defined() && records({&c.slopes})) return py::none();
+  const bool table_grad = c.table.defined() && records({&c.table});
+  const bool grad = table_grad || records({&q, &k, &v});
+  if (grad && !(dense(q) && dense(k) && dense(v))) return py::none();
+  py::gil_scoped_release nogil;
+  Tensor o;
+  if (grad) {
+    o = BiasedFunction::apply(q, k, v, optional(c.table), optional(docs), optional(prefix), optional(c.slopes), sm_scale,
+                              c.softcap, (int64_t)c.max_distance, (int64_t)(table_grad ? c.buckets() : 0));
+  } else {
+    at::AutoDispatchBelowADInplaceOrView below;
+    o = biased_forward(q, k, v, docs, prefix, c, sm_scale, -1).o;
+  }
+  py::gil_scoped_acquire gil;
+  return py::reinterpret_steal<py::object>(THPVariable_Wrap(o));
+}
+
+// Fields of a KVSegment object as the kernels take them.
+struct Segment {
+  Tensor k, v, len;
+  int64_t scan;
+};
+
+bool read_segment(py::handle seg, int64_t b, int64_t h, int64_t d, at::ScalarType type, c10::Device device, Segment& s) {
+  static PyObject* const names[4] = {PyUnicode_InternFromString("k"), PyUnicode_InternFromString("v"),
+                                     PyUnicode_InternFromString("lengths"), PyUnicode_InternFromString("max_len_cap")};
+  py::object f[4];
+  for (int j = 0; j < 4; ++j) {
+    f[j] = py::reinterpret_steal<py::object>(PyObject_GetAttr(seg.ptr(), names[j]));
+    if (!f[j]) {
+      PyErr_Clear();
+      return false;
+    }
+  }
+  s.k = plain(f[0]);
+  s.v = plain(f[1]);
+  s.len = plain(f[2]);
+  for (const Tensor* t : {&s.k, &s.v, &s.len})
+    if (!t->defined() || t->device() != device) return false;
+  if (s.k.scalar_type() != type || s.v.scalar_type() != type || s.k.dim() != 4 || s.v.sizes() != s.k.sizes() ||
+      s.k.size(0) != b || s.k.size(1) != h || s.k.size(3) != d || !fits_int(s.k.size(2)) || !rows16(s.k) ||
+      !rows16(s.v) || s.k.stride(2) < 0 || s.v.stride(2) < 0 || index_code(s.len.scalar_type()) < 0)
+    return false;
+  const bool per_head = s.len.dim() == 2;
+  if (per_head ? (s.len.size(0) != b || s.len.size(1) != h) : (s.len.dim() != 1 || s.len.size(0) != b)) return false;
+  s.scan = s.k.size(2);
+  if (!f[3].is_none()) {
+    const auto cap = as_int(f[3]);
+    if (!cap || *cap < 0) return false;
+    if (s.scan > 0) s.scan = std::max<int64_t>(1, std::min<int64_t>(s.scan, *cap));
+  }
+  return true;
+}
+
+// A [B, T, H, D] tensor of the drafts readable in place.
+bool draft_rows(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, c10::Device device) {
+  return t.defined() && t.scalar_type() == type && t.device() == device && t.sizes() == sizes && rows16(t) &&
+         t.stride(1) >= 0;
+}
+
+bool read_parents(py::handle parents_, int64_t b, int64_t t, c10::Device device, Tensor& parents) {
+  if (parents_.is_none()) return true;
+  parents = plain(parents_);
+  return parents.defined() && parents.dim() == 2 && parents.size(0) == b && parents.size(1) == t &&
+         index_code(parents.scalar_type()) >= 0 && parents.is_contiguous() && parents.device() == device;
+}
+
+py::object tree_attention(py::handle q_, py::handle segments_, py::handle dk_, py::handle dv_, py::handle parents_,
+                          py::handle scale_, py::handle softcap_, py::handle slopes_, py::handle table_,
+                          py::handle max_distance_) {
+  if (!plain_thread() || !PyList_Check(segments_.ptr()) ||
+      !(scale_.is_none() || PyFloat_CheckExact(scale_.ptr()) || PyLong_CheckExact(scale_.ptr())))
+    return py::none();
+  const Tensor q = plain(q_), dk = plain(dk_), dv = plain(dv_);
+  if (!q.defined() || q.dim() != 4 || q.numel() == 0) return py::none();
+  const int64_t b = q.size(0), t = q.size(1), h = q.size(2), d = q.size(3);
+  const auto type = q.scalar_type();
+  double scale = 1.0 / std::sqrt((double)d);
+  if (!scale_.is_none()) scale = PyFloat_AsDouble(scale_.ptr());
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return py::none();
+  }
+  if ((type != at::kBFloat16 && type != at::kHalf) || t > 64 || b > 65535 || h > 65535 || !decode_head_dim(d) ||
+      !std::isfinite((float)scale) || !draft_rows(q, q.sizes(), type, q.device()) ||
+      !draft_rows(dk, q.sizes(), type, q.device()) || !draft_rows(dv, q.sizes(), type, q.device()) ||
+      records({&q, &dk, &dv}))
+    return py::none();
+  Tensor parents;
+  Change c;
+  const py::list segments = py::reinterpret_borrow<py::list>(segments_);
+  const int n_seg = (int)segments.size();
+  if (n_seg > 3 || !read_parents(parents_, b, t, q.device(), parents) ||
+      !read_change(softcap_, slopes_, table_, max_distance_, h, q.device(), c) ||
+      (c.slopes.defined() && records({&c.slopes})))
+    return py::none();
+  Segment seg[3];
+  const void *sk[3], *sv[3], *sl[3];
+  int64_t skst[9], svst[9], scan[3];
+  int ldt[3], lph[3];
+  for (int i = 0; i < n_seg; ++i) {
+    if (!read_segment(segments[i], b, h, d, type, q.device(), seg[i]) || !seg[i].len.is_contiguous()) return py::none();
+    sk[i] = seg[i].k.data_ptr();
+    sv[i] = seg[i].v.data_ptr();
+    sl[i] = seg[i].len.data_ptr();
+    scan[i] = seg[i].scan;
+    ldt[i] = index_code(seg[i].len.scalar_type());
+    lph[i] = seg[i].len.dim() == 2;
+    for (int j = 0; j < 3; ++j) {
+      skst[3 * i + j] = seg[i].k.stride(j);
+      svst[3 * i + j] = seg[i].v.stride(j);
+    }
+  }
+  Tensor out;
+  {
+    py::gil_scoped_release nogil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::DeviceGuard on_device(q.device());
+    out = at::empty(q.sizes(), q.options());
+    const size_t bytes = sps_tree_workspace_bytes((int)b, (int)h, (int)d, (int)t, n_seg, scan);
+    const Tensor ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+    const sps_score_change change = c.args();
+    check("sps_tree_attention",
+          sps_tree_attention((int)b, (int)h, (int)d, (int)t, float_code(type), q.data_ptr(), q.strides().data(), n_seg, sk,
+                             skst, sv, svst, sl, ldt, lph, scan, dk.data_ptr(), dk.strides().data(), dv.data_ptr(),
+                             dv.strides().data(), parents.defined() ? parents.data_ptr() : nullptr,
+                             parents.defined() ? index_code(parents.scalar_type()) : SPS_DTYPE_I32, t, (float)scale,
+                             &change, out.data_ptr(), ws.data_ptr(), bytes, stream_of(q)));
+  }
+  return py::reinterpret_steal<py::object>(THPVariable_Wrap(out));
+}
+
+// commit_drafts; false: the caller takes the general path.
+bool commit_drafts(py::handle segment_, py::handle dk_, py::handle dv_, py::handle last_, py::handle parents_) {
+  if (!plain_thread()) return false;
+  const Tensor dk = plain(dk_), dv = plain(dv_), last = plain(last_);
+  if (!dk.defined() || dk.dim() != 4 || dk.numel() == 0 || !last.defined()) return false;
+  const int64_t b = dk.size(0), t = dk.size(1), h = dk.size(2), d = dk.size(3);
+  const auto type = dk.scalar_type();
+  Segment s;
+  Tensor parents;
+  if (float_code(type) < 0 || t > 64 || b > 65535 || h > 65535 || !decode_head_dim(d) ||
+      !read_segment(segment_, b, h, d, type, dk.device(), s) || !draft_rows(dk, dk.sizes(), type, dk.device()) ||
+      !draft_rows(dv, dk.sizes(), type, dk.device()) || !read_parents(parents_, b, t, dk.device(), parents) ||
+      last.dim() != 1 || last.size(0) != b || index_code(last.scalar_type()) < 0 || !last.is_contiguous() ||
+      last.device() != dk.device())
+    return false;
+  const bool per_head = s.len.dim() == 2;
+  const int64_t kvst[6] = {s.k.stride(0), s.k.stride(1), s.k.stride(2), s.v.stride(0), s.v.stride(1), s.v.stride(2)};
+  const int64_t lst[2] = {s.len.stride(0), per_head ? s.len.stride(1) : 0};
+  c10::DeviceGuard on_device(dk.device());
+  void* stream = stream_of(dk);
+  py::gil_scoped_release nogil;
+  check("sps_commit_drafts",
+        sps_commit_drafts((int)b, (int)h, (int)d, (int)t, float_code(type), s.k.data_ptr(), s.v.data_ptr(), kvst,
+                          (int)s.k.size(2), s.len.data_ptr(), index_code(s.len.scalar_type()), per_head, lst,
+                          dk.data_ptr(), dk.strides().data(), dv.data_ptr(), dv.strides().data(),
+                          parents.defined() ? parents.data_ptr() : nullptr,
+                          parents.defined() ? index_code(parents.scalar_type()) : SPS_DTYPE_I32, t, last.data_ptr(),
+                          index_code(last.scalar_type()), stream));
+  return true;
+}
+
+// ---------------------------------------------------------------------------------------------
 // RoPE.
 // ---------------------------------------------------------------------------------------------
 bool rope_readable(const Tensor& t) { return rows16(t); }
@@ -642,4 +1002,7 @@ PYBIND11_MODULE(_torch_binding, m) {
   m.def("rope", &rope);
   m.def("kv_update", &kv_update);
   m.def("decode", &decode);
+  m.def("biased_attention", &biased_attention);
+  m.def("tree_attention", &tree_attention);
+  m.def("commit_drafts", &commit_drafts);
 }

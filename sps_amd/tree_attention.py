@@ -95,6 +95,12 @@ def tree_attention(
     share one dtype; segments need not be contiguous. ``sm_scale``: 1 / sqrt(D) by default. ``softcap``, ``slopes``,
     ``bias_table``, ``max_distance``: as in ``biased_attention``; positions run through the segments' live keys in
     their order, and a draft's position is their number plus its depth. Forward only (no gradients)."""
+    if not torch.compiler.is_compiling():
+        # Ordinary eager calls run in native code; None: the general path below.
+        out = N.binding().tree_attention(q_BxTxHxD, segments, draft_k_BxTxHxD, draft_v_BxTxHxD, parents_BxT, sm_scale,
+                                         softcap, slopes, bias_table, max_distance)
+        if out is not None:
+            return out
     if not q_BxTxHxD.is_cuda:
         raise RuntimeError("sps_amd tree_attention runs on the GPU only (got a CPU tensor)")
     if q_BxTxHxD.dim() != 4:
@@ -155,6 +161,9 @@ def commit_drafts(
     order, and the lengths ([B] or [B, H]) advance by the rows stored. Rows past the storage are dropped and
     the length stops there. Nothing happens where ``last_B`` names no draft (-1, out of range, padding) or
     a length is negative or already at the end. Drafts have the caches' dtype (bf16, f16 or fp32)."""
+    if not torch.compiler.is_compiling() and N.binding().commit_drafts(segment, draft_k_BxTxHxD, draft_v_BxTxHxD, last_B,
+                                                                       parents_BxT):
+        return
     if not segment.k.is_cuda:
         raise RuntimeError("sps_amd commit_drafts runs on the GPU only (got a CPU tensor)")
     if draft_k_BxTxHxD.dim() != 4:
