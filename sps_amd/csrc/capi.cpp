@@ -526,7 +526,7 @@ int64_t tree_chunks(int n_seg, const int64_t* scan, int chunk) {
 }
 
 size_t tree_part_bytes(int B, int H, int D, int T, int64_t chunks) {
-  return align_up((size_t)B * H * (chunks + 1) * T * sps::tree_record_floats(D) * sizeof(float));
+  return align_up((size_t)B * H * (chunks > 0 ? chunks : 1) * T * sps::tree_record_floats(D) * sizeof(float));
 }
 
 }  // namespace
@@ -539,7 +539,7 @@ size_t sps_tree_workspace_bytes(int B, int H, int D, int T, int n_seg, const int
     return 0;
   for (int s = 0; s < n_seg; ++s)
     if (seg_scan[s] < 0) return 0;
-  const int chunk = sps::tree_chunk_keys(B, H, D, T, n_seg, seg_scan);
+  const int chunk = sps::tree_chunk_keys(B, H, T, n_seg, seg_scan);
   return tree_part_bytes(B, H, D, T, tree_chunks(n_seg, seg_scan, chunk));
 }
 
@@ -577,7 +577,7 @@ int sps_tree_attention(int B, int H, int D, int T, int dtype, const void* q, con
   sps::TreeArgs a;
   std::memset(static_cast<void*>(&a), 0, sizeof(a));
   // A workspace for larger sizes may be too small for this call's own, shorter chunks: longer ones serve then.
-  int chunk = sps::tree_chunk_keys(B, H, D, T, n_seg, seg_scan);
+  int chunk = sps::tree_chunk_keys(B, H, T, n_seg, seg_scan);
   while (workspace_bytes < tree_part_bytes(B, H, D, T, tree_chunks(n_seg, seg_scan, chunk)) && chunk < 4096) chunk *= 2;
   const int64_t chunks = tree_chunks(n_seg, seg_scan, chunk);
   const size_t need = tree_part_bytes(B, H, D, T, chunks);

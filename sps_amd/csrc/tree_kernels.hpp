@@ -10,8 +10,6 @@ namespace sps {
 
 constexpr int kMaxDrafts = 64;
 
-// Keys a workgroup stages per step (groups of 32-key blocks, double-buffered).
-constexpr int tree_group(int D) { return D >= 256 ? 2 : 4; }
 // Floats per partial record of one query: acc[D], max, sum, 2 pad.
 constexpr int tree_record_floats(int D) { return D + 4; }
 
@@ -35,7 +33,7 @@ struct TreeArgs {
   const void* parents;    // [B, T] int32 or int64 (unit stride along T), or null: a chain
   int parents_i64;
   int64_t parents_sb;
-  float* part;   // [B H, n_chunks + 1, T, D + 4]: chunk records, then the drafts' own
+  float* part;   // [B H, max(n_chunks, 1), T, D + 4]: the chunks' records
   int n_chunks, chunk_keys;
   uint16_t* out;  // [B, T, H, D] contiguous
   int cap, bias;  // scores capped / biased
@@ -45,7 +43,7 @@ struct TreeArgs {
 hipError_t launch_tree(const TreeArgs& a, int D, int is_f16, hipStream_t stream);
 
 // Keys per chunk and workgroup, from the sizes the host knows.
-int tree_chunk_keys(int B, int H, int D, int T, int n_seg, const int64_t* scan);
+int tree_chunk_keys(int B, int H, int T, int n_seg, const int64_t* scan);
 
 struct CommitArgs {
   int B, H, T;
