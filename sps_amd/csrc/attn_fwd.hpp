@@ -66,6 +66,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(W, 8))) voi
   // padded tiles.
   constexpr bool kDma = D >= 64;
   using DT = DmaTile<kDma ? D : 64, false>;
+  using DK = DmaTile<kDma ? D : 64, M::kOn && D == 128>;  // K's tiles: see row_frag
   constexpr int TE = kDma ? DT::ELEMS : G::ELEMS;
   // One array per buffer ([block of the pair]): every use names its buffer with a compile-time
   // index, so the compiler can tell the buffers apart, and the score-tile reads of one buffer do not
@@ -105,10 +106,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(W, 8))) voi
   // scores, so the scale must be positive: a negative sm_scale flips the sign of Q instead (exact in
   // bf16/f16: S * scale2 = (-S) * (-scale2)), and a zero one becomes 2^-100 (every visible score
   // scales to within 2^-80 of 0, as with scale 0, while masked ones stay -inf).
-  // (Changed scores come out of the change in the log2 domain: nothing to scale after it.)
+  // (Changed scores come out of the change in the log2 domain: nothing to scale after it. Capped ones without a bias
+  // stay -r through the softmax instead, in units of 2 cap log2 e and cap log2 e below the scores: the running maximum
+  // is then subtracted in the FMA that scales them, as for plain scores.)
+  constexpr bool kRatio = M::kCap && !M::kBias;
   const bool flip_q = !M::kOn && a.scale2 < 0.f;
-  const float scale2 = M::kOn ? 1.f : flip_q ? -a.scale2 : (a.scale2 == 0.f ? 0x1p-100f : a.scale2);
   const ScoreConsts consts = score_consts<M>(a, h);
+  const float scale2 = kRatio ? 2.f * consts.cap2 : M::kOn ? 1.f : flip_q ? -a.scale2 : (a.scale2 == 0.f ? 0x1p-100f : a.scale2);
   float* lut = nullptr;
   if constexpr (M::kBias) {
     lut = dynamic_lds();
@@ -172,21 +176,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(W, 8))) voi
   };
   // LDS-DMA staging. The second block of a last pair that has only one reads as zeros: its scores
   // are masked, and its V rows must be finite for the zero-weighted PV product.
-  const auto k_dma = DT::sources(tid, (uint32_t)(step * a.sk.n * 2));
+  const auto k_dma = DK::sources(tid, (uint32_t)(step * a.sk.n * 2));
   const auto v_dma = DT::sources(tid, (uint32_t)(step * a.sv.n * 2));
   auto issue_dma = [&](int j, int buf) {
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
       const int i = 2 * j + y;
       const bool s0 = i < plan.n0, in = i < nb;
-      DT::load(k_src, in ? (uint32_t)i * k_blk + (s0 ? k_c0 : k_c1) : kOutOfRange, k_dma, tK(buf, y), wave);
+      DK::load(k_src, in ? (uint32_t)i * k_blk + (s0 ? k_c0 : k_c1) : kOutOfRange, k_dma, tK(buf, y), wave);
       DT::load(v_src, in ? (uint32_t)i * v_blk + (s0 ? v_c0 : v_c1) : kOutOfRange, v_dma, tV(buf, y), wave);
     }
   };
-  // Fragment reads of a staged key block.
+  // Fragment reads of a staged key block. (K is only read by rows, so at D = 128 the conflict-free swizzle costs it four
+  // address registers, which changed scores have left; the unchanged ones keep the lean one they were tuned with.)
   auto row_frag = [&](const uint16_t* tile, int c) {
     if constexpr (kDma)
-      return lds_read_b128(tile + DT::frag(c32, g, c));
+      return lds_read_b128(tile + DK::frag(c32, g, c));
     else
       return lds_read_b128(tile + c32 * G::RS + 16 * c + 8 * g);
   };
@@ -233,7 +238,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(W, 8))) voi
         f32x16_t sc = E::mfma(row_frag(kt, 0), qf[0], f32x16_t{});
 #pragma unroll
         for (int c = 1; c < D / 16; ++c) sc = E::mfma(row_frag(kt, c), qf[c], sc);
-        if constexpr (M::kOn) {
+        if constexpr (kRatio) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sc[e] = __builtin_amdgcn_rcpf(-1.f - fast_exp2(sc[e] * consts.cap_in));
+        } else if constexpr (M::kOn) {
           const int q0 = tp.tile * kTile + wave * kBlock, t0 = plan.first(2 * j + y);
           const BlockKind kind = block_kind(wave_uniform(q0 - t0 - 31), consts.far);
           qs_scores<M>(sc, consts, lut, qp, t0, g, kind, 0.f, [](int, float) {});
@@ -276,9 +284,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(W, 8))) voi
           const float p0 = fast_exp2(__builtin_fmaf(sc[2 * e], scale2, negm));
           const float p1 = fast_exp2(__builtin_fmaf(sc[2 * e + 1], scale2, negm));
           pk[e] = E::pack2(p0, p1);
-          // Four independent partial sums, of the rounded weights; with changed scores of the unrounded ones, since
-          // the bias table's gradient may be kept in 32 bits and its weights come from this log-sum-exp.
-          if constexpr (M::kOn)
+          // Four independent partial sums, of the rounded weights; with a bias of the unrounded ones, since the
+          // gradient of its table may be kept in 32 bits and the weights for it come from this log-sum-exp.
+          if constexpr (M::kBias)
             l_run[e & 3] += p0 + p1;
           else
             l_run[e & 3] = E::sum2(pk[e], l_run[e & 3]);
@@ -335,6 +343,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(W, 8))) voi
         }
       }
     }
+    if constexpr (kRatio) m_run += consts.cap2;
     if (g == 0) a.lse[((int64_t)b * a.H + h) * m.N + qp] = l_tot > 0.f ? m_run + __log2f(l_tot) : -INFINITY;
   }
 }
