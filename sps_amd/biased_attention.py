@@ -20,7 +20,6 @@ with the relative error of that rounding, not of fp32. Results do not depend on 
 from __future__ import annotations
 
 import ctypes as C
-import math
 from typing import Optional, Tuple
 
 import torch
@@ -30,6 +29,7 @@ from . import _native as N
 from .attention import _alloc_like_bnhd, _docs_args, _dtype_code, _kernel_view, _strides, _stream, _validate, _ws_args
 
 _TABLE_DTYPES = {torch.bfloat16: N.DTYPE_BF16, torch.float16: N.DTYPE_F16, torch.float32: N.DTYPE_F32}
+MIN_CAP, MAX_CAP = 2.0 ** -10, 2.0 ** 20
 _LEN_DTYPES = {torch.int32: N.DTYPE_I32, torch.int64: N.DTYPE_I64}
 
 
@@ -49,8 +49,8 @@ def bias_buckets(distances: int, num_buckets: int, max_distance: int = 128) -> T
 def check_change(softcap: Optional[float], slopes: Optional[Tensor], bias_table: Optional[Tensor], max_distance: int,
                  n_head: int, device: torch.device) -> float:
     """Validates the score changes of a call with ``n_head`` heads; returns the cap (0 for none)."""
-    if softcap is not None and not (math.isfinite(softcap) and softcap > 0):
-        raise ValueError(f"softcap must be a positive finite number or None, got {softcap}")
+    if softcap is not None and not MIN_CAP <= softcap <= MAX_CAP:
+        raise ValueError(f"softcap must be None or in [2^-10, 2^20], got {softcap}")
     if slopes is not None:
         if slopes.dtype != torch.float32:
             raise TypeError(f"slopes must be float32, got {slopes.dtype}")
@@ -197,7 +197,8 @@ def biased_attention(
     """Document-masked causal attention with changed scores. q, k, v: [B, H, T, D] bf16/f16, D in 16 .. 256 as
     ``full_attention``; returns [B, H, T, D] (in [B, T, H, D] memory order).
 
-    ``softcap``: scores are capped to (-softcap, softcap) by a tanh. ``slopes``: [H] fp32, the scores lose
+    ``softcap``: scores are capped to (-softcap, softcap) by a tanh, in fp32: 2^-10 to 2^20, and an error of the scores
+    of some 2^-22 softcap, so a great cap is better left out. ``slopes``: [H] fp32, the scores lose
     slopes[h] times the distance; no gradient. ``bias_table``: [num_buckets, H] bf16/f16/fp32, added by distance bucket
     (``bias_buckets``); entries below -16384 (-inf, the types' lowest values) hide their pairs.
     ``documents_idx_BxT``: [B, T] ids as in ``full_attention``. ``prefix_len_B``: [B] int32/int64, the leading

@@ -22,6 +22,7 @@
 namespace sps {
 
 constexpr int kMaxDistance = 512;    // largest distance a bucket may start at
+constexpr float kMinCap = 0x1p-10f, kMaxCap = 0x1p20f;  // caps outside lose the scores to fp32's range or precision
 constexpr int kMaxBuckets = 256;
 constexpr int kLutPad = 64;          // a block's distances span 63, on either side of [0, far]
 constexpr float kHidden = -16384.f;  // (their log-sum-exp would leave fp32 no bits for the scores)

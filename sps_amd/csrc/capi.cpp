@@ -330,7 +330,8 @@ void distance_buckets(int buckets, int M, uint16_t* first, uint8_t* bucket, int&
 
 int check_change(const sps_score_change* c) {
   if (!c) return fail(SPS_E_INVALID, "change: null pointer");
-  if (!(std::isfinite(c->softcap) && c->softcap >= 0.f)) return fail(SPS_E_INVALID, "softcap must be 0 or a positive finite number");
+  if (c->softcap != 0.f && !(c->softcap >= sps::kMinCap && c->softcap <= sps::kMaxCap))
+    return fail(SPS_E_INVALID, "softcap must be 0 or in [2^-10, 2^20]");
   if (!c->bias_table) return SPS_OK;
   if (c->table_dtype != SPS_DTYPE_BF16 && c->table_dtype != SPS_DTYPE_F16 && c->table_dtype != SPS_DTYPE_F32)
     return fail(SPS_E_UNSUPPORTED, "bias table dtype code %d not supported (bf16, f16, fp32)", c->table_dtype);
@@ -339,6 +340,11 @@ int check_change(const sps_score_change* c) {
   if (c->max_distance <= c->num_buckets / 2 || c->max_distance > sps::kMaxDistance)
     return fail(SPS_E_UNSUPPORTED, "max_distance %d not in (num_buckets / 2, %d]", c->max_distance, sps::kMaxDistance);
   return SPS_OK;
+}
+
+// Every product of the scale with the smallest cap's constants is finite.
+int check_scale(float sm_scale) {
+  return std::fabs(sm_scale) <= 1e30f ? SPS_OK : fail(SPS_E_INVALID, "sm_scale must be finite and at most 1e30");
 }
 
 // The score fields of the argument block from a checked change.
@@ -368,7 +374,7 @@ int check_biased(const char* prefix_name, const void* prefix, int prefix_dtype, 
   if (!supported_head_dim(D)) return fail(SPS_E_UNSUPPORTED, "head_dim %d not supported", D);
   if (dtype != SPS_DTYPE_BF16 && dtype != SPS_DTYPE_F16)
     return fail(SPS_E_UNSUPPORTED, "attention dtype code %d not supported (bf16, f16)", dtype);
-  if (!std::isfinite(sm_scale)) return fail(SPS_E_INVALID, "sm_scale must be finite");
+  if (const int rc = check_scale(sm_scale)) return rc;
   return SPS_OK;
 }
 
@@ -519,6 +525,18 @@ int check_drafts(int B, int H, int D, int T) {
   return SPS_OK;
 }
 
+// The bytes from the first to the last element of rows of D elements.
+struct Extent {
+  intptr_t lo, hi;
+  bool meets(const Extent& o) const { return lo < o.hi && o.lo < hi; }
+};
+Extent extent(const void* p, const int64_t* st, int n0, int n1, int n2, int D, int bytes) {
+  Extent e{reinterpret_cast<intptr_t>(p), reinterpret_cast<intptr_t>(p) + (intptr_t)D * bytes};
+  const int n[3] = {n0, n1, n2};
+  for (int i = 0; i < 3; ++i) (st[i] < 0 ? e.lo : e.hi) += (intptr_t)(n[i] - 1) * st[i] * bytes;
+  return e;
+}
+
 int64_t tree_chunks(int n_seg, const int64_t* scan, int chunk) {
   int64_t n = 0;
   for (int s = 0; s < n_seg; ++s) n += (scan[s] + chunk - 1) / chunk;
@@ -556,7 +574,7 @@ int sps_tree_attention(int B, int H, int D, int T, int dtype, const void* q, con
   if (rc) return rc;
   if (dtype != SPS_DTYPE_BF16 && dtype != SPS_DTYPE_F16)
     return fail(SPS_E_UNSUPPORTED, "tree attention dtype code %d not supported (bf16, f16)", dtype);
-  if (!std::isfinite(sm_scale)) return fail(SPS_E_INVALID, "sm_scale must be finite");
+  if ((rc = check_scale(sm_scale))) return rc;
   if (n_seg < 0 || n_seg > sps::kMaxDecodeSegs)
     return fail(SPS_E_INVALID, "at most %d segments (got %d)", sps::kMaxDecodeSegs, n_seg);
   const sps_score_change none = {};
@@ -660,6 +678,20 @@ int sps_commit_drafts(int B, int H, int D, int T, int dtype, void* k, void* v, c
       (rc = check_rows("draft_v", draft_v, draft_v_strides, bytes)))
     return rc;
   if (!len || !last) return fail(SPS_E_INVALID, "lengths or last: null pointer");
+  // What is written must be of one place each, and not what is read.
+  for (int i = 0; i < 6; i += 3)
+    if ((B > 1 && !kv_strides[i]) || (H > 1 && !kv_strides[i + 1]) ||
+        (storage > 1 && std::llabs((long long)kv_strides[i + 2]) < D))
+      return fail(SPS_E_INVALID, "the cache's rows overlap: a view of its own memory expanded");
+  if ((B > 1 && !len_strides[0]) || (len_per_head && H > 1 && !len_strides[1]))
+    return fail(SPS_E_INVALID, "the lengths overlap: an expanded view");
+  if (k == v) return fail(SPS_E_INVALID, "keys and values share their memory");
+  for (int i = 0; i < 2; ++i) {
+    const Extent cache = extent(i ? v : k, kv_strides + 3 * i, B, H, storage, D, bytes);
+    for (int j = 0; j < 2; ++j)
+      if (cache.meets(extent(j ? draft_v : draft_k, j ? draft_v_strides : draft_k_strides, B, T, H, D, bytes)))
+        return fail(SPS_E_INVALID, "the drafts lie within the cache's memory: pass copies");
+  }
   sps::CommitArgs a;
   std::memset(&a, 0, sizeof(a));
   a.B = B;

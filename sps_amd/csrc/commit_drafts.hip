@@ -37,8 +37,9 @@ __global__ __launch_bounds__(kCommitThreads) void commit_kernel(const CommitArgs
   const int pieces = a.row_bytes / 16, total = nh * n * pieces;
   for (int i = tid; i < total; i += kCommitThreads) {
     const int p = i % pieces, r = i / pieces, j = r % n, h = h0 + r / n;
-    const int64_t at = length(h) + j;
-    if (at - j < 0 || at >= a.storage) continue;
+    const int64_t len = length(h);
+    if (len < 0 || len >= a.storage - j) continue;
+    const int64_t at = len + j;
     const int t = s_path[j];
     const u32x4_t kx = *reinterpret_cast<const u32x4_t*>(a.dk + b * a.dk_sb + t * a.dk_st + h * a.dk_sh + 16 * p);
     const u32x4_t vx = *reinterpret_cast<const u32x4_t*>(a.dv + b * a.dv_sb + t * a.dv_st + h * a.dv_sh + 16 * p);
@@ -49,7 +50,7 @@ __global__ __launch_bounds__(kCommitThreads) void commit_kernel(const CommitArgs
   for (int i = tid; i < (a.len_per_head ? nh : 1); i += kCommitThreads) {
     const int64_t len = length(h0 + i);
     if (len < 0 || len >= a.storage) continue;
-    const int64_t to = len + n < a.storage ? len + n : a.storage;
+    const int64_t to = len < a.storage - n ? len + n : a.storage;
     cache_len_store(a.len, b * a.len_sb + (a.len_per_head ? (h0 + i) * a.len_sh : 0), a.len_i64, to);
   }
 }

@@ -322,7 +322,7 @@ bool read_change(py::handle softcap, py::handle slopes, py::handle table, py::ha
       PyErr_Clear();
       return false;
     }
-    if (!std::isfinite((float)c.softcap) || !((float)c.softcap > 0.f)) return false;
+    if (!(c.softcap >= 0x1p-10 && c.softcap <= 0x1p20)) return false;
   }
   if (!slopes.is_none()) {
     c.slopes = plain(slopes);
@@ -566,14 +566,16 @@ py::object tree_attention(py::handle q_, py::handle segments_, py::handle dk_, p
   const int n_seg = (int)segments.size();
   if (n_seg > 3 || !read_parents(parents_, b, t, q.device(), parents) ||
       !read_change(softcap_, slopes_, table_, max_distance_, h, q.device(), c) ||
-      (c.slopes.defined() && records({&c.slopes})))
+      (c.slopes.defined() && records({&c.slopes})) || (c.table.defined() && records({&c.table})))
     return py::none();
   Segment seg[3];
   const void *sk[3], *sv[3], *sl[3];
   int64_t skst[9], svst[9], scan[3];
   int ldt[3], lph[3];
   for (int i = 0; i < n_seg; ++i) {
-    if (!read_segment(segments[i], b, h, d, type, q.device(), seg[i]) || !seg[i].len.is_contiguous()) return py::none();
+    if (!read_segment(segments[i], b, h, d, type, q.device(), seg[i]) || !seg[i].len.is_contiguous() ||
+        records({&seg[i].k, &seg[i].v}))
+      return py::none();
     sk[i] = seg[i].k.data_ptr();
     sv[i] = seg[i].v.data_ptr();
     sl[i] = seg[i].len.data_ptr();

@@ -101,6 +101,13 @@ def tree_attention(
                                          softcap, slopes, bias_table, max_distance)
         if out is not None:
             return out
+    return _tree_attention(q_BxTxHxD, segments, draft_k_BxTxHxD, draft_v_BxTxHxD, parents_BxT, sm_scale, softcap, slopes,
+                           bias_table, max_distance)
+
+
+@torch.compiler.disable  # compiled models call it as it is: a launch, and views of memory that is updated in place
+def _tree_attention(q_BxTxHxD, segments, draft_k_BxTxHxD, draft_v_BxTxHxD, parents_BxT, sm_scale, softcap, slopes,
+                    bias_table, max_distance) -> Tensor:
     if not q_BxTxHxD.is_cuda:
         raise RuntimeError("sps_amd tree_attention runs on the GPU only (got a CPU tensor)")
     if q_BxTxHxD.dim() != 4:
@@ -115,7 +122,8 @@ def tree_attention(
         raise ValueError(f"tree_attention is built for head_dim in {_DECODE_HEAD_DIMS}, got {d}")
     if len(segments) > 3:
         raise ValueError(f"tree_attention takes at most 3 segments, got {len(segments)}")
-    if torch.is_grad_enabled() and any(x.requires_grad for x in (q_BxTxHxD, draft_k_BxTxHxD, draft_v_BxTxHxD)):
+    read = [q_BxTxHxD, draft_k_BxTxHxD, draft_v_BxTxHxD, *(x for sg in segments for x in (sg.k, sg.v))]
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (*read, bias_table)):
         raise RuntimeError("tree_attention has no backward: call it under torch.no_grad() or on detached tensors")
     q = _drafts("queries", q_BxTxHxD, shape, dtype, device)
     dk = _drafts("draft keys", draft_k_BxTxHxD, shape, dtype, device)
@@ -160,10 +168,16 @@ def commit_drafts(
     ``last_B``: [B] int32/int64, the last accepted draft of each sequence; the path from its root to it is appended in
     order, and the lengths ([B] or [B, H]) advance by the rows stored. Rows past the storage are dropped and
     the length stops there. Nothing happens where ``last_B`` names no draft (-1, out of range, padding) or
-    a length is negative or already at the end. Drafts have the caches' dtype (bf16, f16 or fp32)."""
+    a length is negative or already at the end. Drafts have the caches' dtype (bf16, f16 or fp32) and memory outside
+    the caches'; caches and lengths are no expanded views."""
     if not torch.compiler.is_compiling() and N.binding().commit_drafts(segment, draft_k_BxTxHxD, draft_v_BxTxHxD, last_B,
                                                                        parents_BxT):
         return
+    _commit_drafts(segment, draft_k_BxTxHxD, draft_v_BxTxHxD, last_B, parents_BxT)
+
+
+@torch.compiler.disable
+def _commit_drafts(segment, draft_k_BxTxHxD, draft_v_BxTxHxD, last_B, parents_BxT) -> None:
     if not segment.k.is_cuda:
         raise RuntimeError("sps_amd commit_drafts runs on the GPU only (got a CPU tensor)")
     if draft_k_BxTxHxD.dim() != 4:
