@@ -141,8 +141,11 @@ class Attention:
             nb, h = self.table.shape
             n = self.q.shape[2]
             e = d_ds + 2.0 ** -24 * (16 + n) * np.abs(self.ds)
+            # A gradient in f16 below 2^-14, its least normal value, is rounded to a multiple of 2^-24: off by up to 2^-25,
+            # whatever its size (1.474e-7 becomes 2 * 2^-24 = 1.192e-7). The other types' steps there are below 2^-126.
+            least = 2.0 ** -25 if table_unit == 2.0 ** -11 else 2.0 ** -126
             out.append(np.stack([[np.where(self._buckets == j, e[:, i], 0.0).sum() for i in range(h)] for j in range(nb)])
-                       + table_unit * np.abs(self.dtable))
+                       + table_unit * np.abs(self.dtable) + least)
         return out
 
 

@@ -40,9 +40,10 @@ HIP_FLAGS = [
     "-amdgpu-mfma-vgpr-form=1",
 ]
 
-SOURCES = ["attn_biased_dq_table.hip", "attn_biased_dq.hip", "attn_biased_fwd.hip", "attn_biased_dkdv.hip",
-           "attn_biased_split.hip", "tree.hip", "commit_drafts.hip", "attn_prep.hip", "attn_fwd.hip", "attn_bwd.hip", "attn_bwd_split.hip", "decode.hip",
-           "kv_update.hip", "rope.hip", "prefill_state.hip", "doc_ids.hip", "capi.cpp"]
+SOURCES = ["attn_biased_dq_table.hip", "attn_biased_dq.hip", "attn_biased_fwd.hip", "attn_biased_few.hip",
+           "attn_biased_dkdv.hip", "attn_biased_split.hip", "tree.hip", "commit_drafts.hip", "attn_prep.hip",
+           "attn_fwd.hip", "attn_bwd.hip", "attn_bwd_split.hip", "decode.hip", "kv_update.hip", "rope.hip",
+           "prefill_state.hip", "doc_ids.hip", "capi.cpp"]
 
 # Per-source flags. The attention kernels are scheduled with LLVM's iterative ILP strategy, which
 # interleaves their MFMA, exponential and LDS work more densely than the default occupancy-driven

@@ -360,6 +360,7 @@ struct TableSums {
 
 // Host launchers.
 hipError_t launch_biased_fwd(const BiasedArgs& a, int D, int is_f16, hipStream_t stream);
+hipError_t launch_biased_fwd_few(const BiasedArgs& a, int D, int is_f16, hipStream_t stream);
 hipError_t launch_biased_dq(const BiasedArgs& a, int D, int is_f16, hipStream_t stream);
 hipError_t launch_biased_dq_table(const BiasedArgs& a, int D, int is_f16, hipStream_t stream);  // fills dtable_part
 hipError_t launch_biased_dkdv(const BiasedArgs& a, int D, int is_f16, hipStream_t stream);
