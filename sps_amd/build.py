@@ -41,6 +41,7 @@ HIP_FLAGS = [
 ]
 
 SOURCES = ["attn_biased_dq_table.hip", "attn_biased_dq.hip", "attn_biased_fwd.hip", "attn_biased_few.hip",
+           "attn_biased_few_bwd.hip",
            "attn_biased_dkdv.hip", "attn_biased_split.hip", "tree.hip", "commit_drafts.hip", "attn_prep.hip",
            "attn_fwd.hip", "attn_bwd.hip", "attn_bwd_split.hip", "decode.hip", "kv_update.hip", "rope.hip",
            "prefill_state.hip", "doc_ids.hip", "capi.cpp"]
@@ -55,6 +56,8 @@ SOURCE_FLAGS = {
     "attn_bwd.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "attn_bwd_split.hip": ["-mllvm", "-amdgpu-use-amdgpu-trackers=1"],
     "attn_biased_fwd.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
+    "attn_biased_few.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
+    "attn_biased_few_bwd.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "attn_biased_dq.hip": ["-mllvm", "-amdgpu-use-amdgpu-trackers=1"],
     "attn_biased_dq_table.hip": ["-mllvm", "-amdgpu-use-amdgpu-trackers=1"],
     "attn_biased_dkdv.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],

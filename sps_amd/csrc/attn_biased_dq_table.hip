@@ -45,7 +45,7 @@ hipError_t launch_biased_dq_table(const BiasedArgs& a, int D, int is_f16, hipStr
 __global__ __launch_bounds__(256) void table_gradient_kernel(const BiasedArgs a, void* out) {
   __shared__ float s_part[256];
   const int h = blockIdx.x, tid = threadIdx.x;
-  const int tiles = q_tiles(a.m.N), nb = a.buckets, shares = 256 / nb;
+  const int tiles = a.dtable_tiles, nb = a.buckets, shares = 256 / nb;
   const int j = tid % nb, share = tid / nb;
   float s = 0.f;
   if (share < shares) {

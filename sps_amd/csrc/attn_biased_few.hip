@@ -3,10 +3,9 @@
 //
 // Scores, masks and softmax as in attn_fwd.hpp. Each wave moves its blocks by itself, through registers into tiles of
 // its own, one block ahead, without barriers (wave_tile.hpp). A chain of latencies bounds such calls, and it is a
-// quarter as long (attn_biased_fwd.hip has the rule and what both forms measured). Per block: the scores' instructions
+// quarter as long (few_tiles, attn_scores.hpp, has the rule and what both forms measured). Per block: the scores' instructions
 // and two dependent product chains, ~1.2 us at one wave per SIMD.
-#include "attn_scores.hpp"
-#include "wave_tile.hpp"
+#include "attn_few.hpp"
 
 namespace sps {
 
@@ -18,8 +17,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_waves<D
     const BiasedArgs a) {
   using W = WaveTile<D>;
   constexpr int DC = TileGeom<D>::DC, TE = kBlock * W::RS;
-  constexpr int AS = D + 4;  // floats per row of the accumulators, which take the tiles' place at the end
-  constexpr int WE = 2 * TE > 64 * AS ? 2 * TE : 64 * AS;
+  constexpr int WE = few_lds<D>();
   __shared__ __attribute__((aligned(16))) uint16_t s_tile[kWaves][WE];
   __shared__ float s_m[kWaves][kBlock], s_l[kWaves][kBlock], s_f[kWaves][kBlock];
 
@@ -65,12 +63,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_waves<D
     __syncthreads();
   }
   uint16_t *const kt = s_tile[wave], *const vt = kt + TE;
-  if constexpr (TileGeom<D>::DPAD > D) {
-    for (int i = lane; i < 2 * kBlock; i += 64) {
-#pragma unroll
-      for (int y = D; y < TileGeom<D>::DPAD; y += 8) lds_write_b128(kt + i * W::RS + y, u32x4_t{0u, 0u, 0u, 0u});
-    }
-  }
+  zero_pads<D>(kt, lane);
 
   float m_run = -INFINITY, l_run[2] = {0.f, 0.f};
   f32x16_t acc[DC];
@@ -128,16 +121,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_waves<D
   }
 
   // The waves join: accumulators through their LDS, each wave's weight once per query.
-  float* const mine = reinterpret_cast<float*>(s_tile[wave]) + c32 * AS;
-#pragma unroll
-  for (int dc = 0; dc < DC; ++dc) {
-#pragma unroll
-    for (int i4 = 0; i4 < 4; ++i4) {
-      const int d = 32 * dc + 8 * i4 + 4 * g;
-      const f32x4_t y = {acc[dc][4 * i4], acc[dc][4 * i4 + 1], acc[dc][4 * i4 + 2], acc[dc][4 * i4 + 3]};
-      if (d < D) *reinterpret_cast<f32x4_t*>(mine + d) = y;
-    }
-  }
+  put_rows<D>(reinterpret_cast<float*>(s_tile[wave]), acc, lane);
   const float l = half_sum(l_run[0] + l_run[1]);
   if (g == 0) {
     s_m[wave][c32] = m_run;
@@ -161,20 +145,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_waves<D
     a.lse[(int64_t)bh * m.N + q0 + tid] = sum > 0.f ? top + __log2f(sum) : -INFINITY;
   }
   __syncthreads();
-  uint16_t* const out = a.out + b * a.sout.b + h * a.sout.h + (int64_t)q0 * a.sout.n;
-  for (int i = tid; i < queries * (D / 8); i += 256) {
-    const int r = i / (D / 8), d = (i % (D / 8)) * 8;
-    float y[8] = {};
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float f = s_f[w][r];
-      const float* x = reinterpret_cast<const float*>(s_tile[w]) + r * AS + d;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = __builtin_fmaf(f, x[e], y[e]);
-    }
-    *reinterpret_cast<u32x4_t*>(out + r * a.sout.n + d) =
-        u32x4_t{E::pack2(y[0], y[1]), E::pack2(y[2], y[3]), E::pack2(y[4], y[5]), E::pack2(y[6], y[7])};
-  }
+  sum_rows<D, E>(reinterpret_cast<const float*>(s_tile[0]), WE / 2, a.out + b * a.sout.b + h * a.sout.h + (int64_t)q0 * a.sout.n,
+                 a.sout.n, queries, tid, [&](int w, int r) { return s_f[w][r]; });
 }
 
 template <int D, class E, class M>

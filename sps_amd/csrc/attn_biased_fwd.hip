@@ -3,17 +3,6 @@
 
 namespace sps {
 
-// Where tiles of 128 queries leave most of the chip idle: 32 queries a workgroup. Its K / V traffic is four times as much,
-// so it loses once the other form fills the CUs. Measured (us, capped; this form against the other): D = 64, 8 heads of
-// 512 tokens 13.6 -> 7.4, of 2048 42 -> 21, 16 of 2048 (256 tiles) 43 -> 28, 32 of 2048 (512) 46 -> 50; D = 128, 32 of 512
-// (128 tiles) 17.6 -> 13.2, 32 of 1024 (256) 31.1 -> 31.5; D = 256, 16 of 512 (64) 25.6 -> 19.2, 32 of 512 (128)
-// 27.3 -> 28.7. With one block of keys there is nothing to split (16 of 32 at D = 128, biased, 6.0 against 6.7). Rows so
-// far apart that offsets of 31 rows past the last would leave 32 bits take the other form.
-static bool few_tiles(const BiasedArgs& a, int D) {
-  return (int64_t)q_tiles(a.m.N) * a.B * a.H <= (D <= 64 ? 256 : D == 128 ? 128 : 64) && a.m.N > kBlock &&
-         a.sk.n < (1 << 24) && a.sv.n < (1 << 24);
-}
-
 template <int D, class E, class M>
 static hipError_t launch_m(const BiasedArgs& a, hipStream_t stream) {
   const int64_t nblocks = (int64_t)q_tiles(a.m.N) * a.B * a.H;

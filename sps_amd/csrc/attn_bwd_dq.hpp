@@ -310,7 +310,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES, 8)))
     run(std::false_type{});
 
   if constexpr (M::kTable)
-    sums.store(a, a.dtable_part + (((int64_t)b * a.H + h) * q_tiles(m.N) + tp.tile) * a.buckets, tid, lane);
+    sums.store(a, a.dtable_part + (((int64_t)b * a.H + h) * a.dtable_tiles + tp.tile) * a.buckets, tid, lane);
 
   uint16_t* orow = a.dq + b * a.sdq.b + h * a.sdq.h + (int64_t)qsafe * a.sdq.n;
   const float sc = a.sm_scale;

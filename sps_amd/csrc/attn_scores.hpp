@@ -28,6 +28,8 @@ constexpr int kLutPad = 64;          // a block's distances span 63, on either s
 constexpr float kHidden = -16384.f;  // (their log-sum-exp would leave fp32 no bits for the scores)
 constexpr float kLog2e = 1.4426950408889634f;
 
+constexpr int kFewTiles = 256;       // at most so many tiles of 128 are few, at any head dim
+
 struct BiasedArgs : AttnArgs {
   const void* prefix;  // [B] int32 or int64: leading positions of each row that all its queries see, or null
   int prefix_i64;
@@ -38,7 +40,8 @@ struct BiasedArgs : AttnArgs {
   int table_dtype;
   int64_t table_sj, table_sh;
   int buckets, far;     // far: first distance of the last bucket
-  float* dtable_part;   // [B, H, q_tiles, buckets]: table gradient of each query tile (backward with a table)
+  float* dtable_part;   // [B, H, dtable_tiles, buckets]: table gradient of each query tile (backward with a table)
+  int dtable_tiles;
   uint8_t bucket[kMaxDistance];      // of the distances below far
   uint16_t first[kMaxBuckets];       // first distance of each bucket (of the next one that has any, where it has none)
 };
@@ -358,9 +361,28 @@ struct TableSums {
   }
 };
 
+// Where tiles of 128 positions leave most of the chip idle, a workgroup has 32. Its traffic is four times as much, so it
+// loses once the other form fills the CUs. Measured (us, capped, the other form against this; rows x heads x tokens):
+//   D = 64   forward 1 x 8 x 512 13.6 / 7.4, 1 x 8 x 2048 42 / 21, 1 x 16 x 2048 (256 tiles) 43 / 28, 2 x 16 x 2048 (512)
+//            46 / 50; dQ at the same 18.5 / 8.9, 55 / 23, 57 / 34; dK/dV 17.2 / 7.8, 58 / 24, 61 / 38, then 70 / 72
+//   D = 128  forward 1 x 8 x 512 17.2 / 9.6, 2 x 16 x 512 (128) 17.6 / 12.0, 1 x 16 x 2048 (256) 55 / 50, 2 x 16 x 1024
+//            (256) 31.1 / 31.5; dQ 26 / 12, 28 / 20, 93 / 72, 4 x 16 x 512 (256) 32 / 38; dK/dV 23 / 12, 25 / 20, 79 / 82
+//   D = 256  forward 2 x 8 x 512 (64) 25.6 / 19.2, 2 x 16 x 512 (128) 27.3 / 28.7; the backward keeps to the other form,
+//            whose wide tiles this one's registers do not hold
+// With one block of 32 there is nothing to split (16 heads of 32 tokens, D = 128, biased, 6.0 against 6.7). Rows so far
+// apart that offsets of 31 rows past the last would leave 32 bits take the other form.
+inline bool few_tiles(const BiasedArgs& a, int D) {
+  const int64_t far = 1 << 24;
+  return (int64_t)q_tiles(a.m.N) * a.B * a.H <= (D <= 64 ? kFewTiles : D == 128 ? 128 : 64) && a.m.N > kBlock &&
+         a.sq.n < far && a.sk.n < far && a.sv.n < far && a.sdo.n < far;
+}
+
 // Host launchers.
 hipError_t launch_biased_fwd(const BiasedArgs& a, int D, int is_f16, hipStream_t stream);
 hipError_t launch_biased_fwd_few(const BiasedArgs& a, int D, int is_f16, hipStream_t stream);
+// The backward's passes where there are few tiles (head dims to 128); dQ with the table's sums where dtable_part is set.
+enum FewPass : int { FEW_DQ, FEW_DKDV };
+hipError_t launch_biased_bwd_few(const BiasedArgs& a, int D, int is_f16, int pass, hipStream_t stream);
 hipError_t launch_biased_dq(const BiasedArgs& a, int D, int is_f16, hipStream_t stream);
 hipError_t launch_biased_dq_table(const BiasedArgs& a, int D, int is_f16, hipStream_t stream);  // fills dtable_part
 hipError_t launch_biased_dkdv(const BiasedArgs& a, int D, int is_f16, hipStream_t stream);

@@ -363,9 +363,10 @@ void set_change(sps::BiasedArgs& a, const sps_score_change& c, float sm_scale, c
   distance_buckets(c.num_buckets, c.max_distance, a.first, a.bucket, a.far);
 }
 
-// Bytes of the query tiles' sums of the table gradient.
+// Bytes of the query tiles' sums of the table gradient (of 32 queries where there may be few tiles).
 size_t table_part_bytes(int B, int H, int N, int num_buckets) {
-  return align_up((size_t)B * H * sps::q_tiles(N) * num_buckets * sizeof(float));
+  const int64_t tiles = (int64_t)B * H * sps::q_tiles(N);
+  return align_up((size_t)tiles * (tiles <= sps::kFewTiles ? sps::kTile / sps::kBlock : 1) * num_buckets * sizeof(float));
 }
 
 int check_biased(const char* prefix_name, const void* prefix, int prefix_dtype, int D, int dtype, float sm_scale) {
@@ -486,15 +487,24 @@ int sps_biased_bwd(int B, int H, int N, int D, int dtype, const void* q, const i
   a.sm_scale = sm_scale;
   a.scale2 = sm_scale * sps::kLog2e;
   set_change(a, *change, sm_scale, prefix_len, prefix_dtype);
+  a.dtable_tiles = sps::q_tiles(N);
   if (dtable) a.dtable_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + part_at);
   const int f16 = dtype == SPS_DTYPE_F16;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (!need) return dtable ? hip_status(sps::launch_table_gradient(a, dtable, s), "bias table gradient") : SPS_OK;
   if (docs && !reuse_layout && (rc = hip_status(sps::launch_row_layout(a, s), "document prepass"))) return rc;
-  if ((rc = hip_status(dtable ? sps::launch_biased_dq_table(a, D, f16, s) : sps::launch_biased_dq(a, D, f16, s),
-                       "biased attention dQ")))
-    return rc;
+  const bool few = D <= 128 && sps::few_tiles(a, D);
+  if (few) {
+    a.dtable_tiles = (N + sps::kBlock - 1) / sps::kBlock;
+    rc = hip_status(sps::launch_biased_bwd_few(a, D, f16, sps::FEW_DQ, s), "biased attention dQ");
+  } else {
+    rc = hip_status(dtable ? sps::launch_biased_dq_table(a, D, f16, s) : sps::launch_biased_dq(a, D, f16, s),
+                    "biased attention dQ");
+  }
+  if (rc) return rc;
   if (dtable && (rc = hip_status(sps::launch_table_gradient(a, dtable, s), "bias table gradient"))) return rc;
+  if (few)
+    return hip_status(sps::launch_biased_bwd_few(a, D, f16, sps::FEW_DKDV, s), "biased attention dK/dV");
   return hip_status(sps::launch_biased_dkdv(a, D, f16, s), "biased attention dK/dV");
 }
 
