@@ -58,6 +58,7 @@ SOURCE_FLAGS = {
     "attn_biased_fwd.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "attn_biased_few.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "attn_biased_few_bwd.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
+    "tree.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "attn_biased_dq.hip": ["-mllvm", "-amdgpu-use-amdgpu-trackers=1"],
     "attn_biased_dq_table.hip": ["-mllvm", "-amdgpu-use-amdgpu-trackers=1"],
     "attn_biased_dkdv.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
