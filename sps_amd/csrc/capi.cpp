@@ -607,7 +607,7 @@ int sps_tree_attention(int B, int H, int D, int T, int dtype, const void* q, con
   // A workspace for larger sizes may be too small for this call's own, shorter chunks: longer ones serve then.
   int chunk = sps::tree_chunk_keys(B, H, T, n_seg, seg_scan);
   while (workspace_bytes < tree_part_bytes(B, H, D, T, tree_chunks(n_seg, seg_scan, chunk)) && chunk < 4096) chunk *= 2;
-  const int64_t chunks = tree_chunks(n_seg, seg_scan, chunk);
+  int64_t chunks = tree_chunks(n_seg, seg_scan, chunk);
   const size_t need = tree_part_bytes(B, H, D, T, chunks);
   if (workspace_bytes < need) return fail(SPS_E_WORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, need);
   if (!workspace) return fail(SPS_E_INVALID, "workspace: null pointer");
@@ -616,7 +616,17 @@ int sps_tree_attention(int B, int H, int D, int T, int dtype, const void* q, con
   a.T = T;
   a.n_seg = n_seg;
   int base = 0;
-  const int64_t most = (int64_t)INT32_MAX / 2 - 1024;  // bytes of a chunk's rows: 32-bit offsets
+  const int64_t most = (int64_t)INT32_MAX / 2 - 1024;  // elements of a chunk's rows: 32-bit byte offsets
+  if (chunks > 1 && sps::tree_whole_rows(B, H, T, n_seg, seg_scan)) {
+    bool fits = true;
+    for (int s = 0; s < n_seg; ++s)
+      fits = fits && (seg_scan[s] == 0 || (seg_k_strides && seg_v_strides && seg_k_strides[3 * s + 2] <= most / keys &&
+                                           seg_v_strides[3 * s + 2] <= most / keys));
+    if (fits) {
+      chunk = (int)keys;
+      chunks = 1;
+    }
+  }
   for (int s = 0; s < n_seg; ++s) {
     sps::TreeSeg& sg = a.seg[s];
     sg.scan = (int)seg_scan[s];

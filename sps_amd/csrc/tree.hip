@@ -285,7 +285,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(tree_waves<
   }
 
   // The waves combine, tile by tile: accumulators through the waves' LDS, each wave's weight once per draft, then one
-  // record per draft, 16 bytes a thread.
+  // record per draft, 16 bytes a thread; or, of a single chunk, the outputs.
+  const bool whole = a.n_chunks <= 1;
   float* out = a.part + ((int64_t)bh * imax(a.n_chunks, 1) + c) * a.T * REC;
 #pragma unroll
   for (int x = 0; x < QW; ++x) {
@@ -319,8 +320,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(tree_waves<
         s_f[s * TS + tile][r] = f;
         L = __builtin_fmaf(f, s_l[s * TS + tile][r], L);
       }
-      out[(q0 + tid) * REC + D] = M;
-      out[(q0 + tid) * REC + D + 1] = first && !s_set[q0 + tid] ? -1.f : L;  // a negative sum marks what is no draft
+      if (whole) {
+        const float inv = L > 0.f ? 1.f / L : 0.f;
+#pragma unroll
+        for (int s = 0; s < SHARES; ++s) s_f[s * TS + tile][r] *= inv;
+      } else {
+        out[(q0 + tid) * REC + D] = M;
+        out[(q0 + tid) * REC + D + 1] = first && !s_set[q0 + tid] ? -1.f : L;  // a negative sum marks what is no draft
+      }
     }
     __syncthreads();
     for (int i = tid; i < drafts * (D / 4); i += 256) {
@@ -334,7 +341,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(tree_waves<
 #pragma unroll
         for (int e = 0; e < 4; ++e) A[e] = __builtin_fmaf(f, y[e], A[e]);
       }
-      *reinterpret_cast<f32x4_t*>(out + (q0 + ql) * REC + d) = A;
+      if (whole) {
+        if (!s_set[q0 + ql]) A = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        *reinterpret_cast<u32x2_t*>(a.out + (((int64_t)b * a.T + q0 + ql) * a.H + h) * D + d) =
+            u32x2_t{E::pack2(A[0], A[1]), E::pack2(A[2], A[3])};
+      } else {
+        *reinterpret_cast<f32x4_t*>(out + (q0 + ql) * REC + d) = A;
+      }
     }
   }
 }
@@ -450,6 +463,24 @@ int tree_chunk_keys(int B, int H, int T, int n_seg, const int64_t* scan) {
   return chunk;
 }
 
+// No merge, no second launch; the rows' lengths are not evened out. For keys in one segment (MI355X, us a call, chunks and
+// merge / whole rows; live lengths 1/2 to 1 of the scan below 2048 keys, 1/8 to 1 from there):
+//  - up to 512 keys always (16 rows, D = 64, one draft, 256 keys 8.8 / 5.5, 512 8.7 / 6.8; 32 rows, D = 128, 61 drafts,
+//    512 17.7 / 16.9), 1024 from 128 rows (16 drafts 13.2 / 12.0; 32 rows, D = 128, one draft 11.0 / 14.0);
+//  - from 256 rows 2048 (D = 128, one draft 37 / 31), which few drafts' calls no longer gain from beyond (4096: 59 / 60);
+//  - with more than eight drafts 4096 (256 rows, D = 64, 16 drafts 32.0 / 32.0, 61 44 / 40; 1024 rows 113 / 108 and
+//    147 / 124), and 8192 from 512 rows (16 drafts 114 / 112, 61 140 / 125).
+bool tree_whole_rows(int B, int H, int T, int n_seg, const int64_t* scan) {
+  const int64_t rows = (int64_t)B * H;
+  int64_t keys = 0;
+  for (int s = 0; s < n_seg; ++s) {
+    if (keys && scan[s]) return false;
+    keys += scan[s];
+  }
+  const int64_t most = rows < 128 ? 512 : rows < 256 ? 1024 : T <= 8 ? 2048 : rows < 512 ? 4096 : 8192;
+  return keys <= most;
+}
+
 template <int D, class E, bool CHANGED>
 static void launch_partial(const TreeArgs& a, hipStream_t stream) {
   const dim3 grid((unsigned)imax(a.n_chunks, 1) * a.B * a.H), block(256);
@@ -467,7 +498,7 @@ static hipError_t launch_t(const TreeArgs& a, hipStream_t stream) {
   else
     launch_partial<D, E, false>(a, stream);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  if (e != hipSuccess || a.n_chunks <= 1) return e;
   const int64_t drafts = (int64_t)a.B * a.H * a.T;
   constexpr int kGroups = 256 / (D / 4);
   // A lane group walks its chunks eight at a time; past that a workgroup shares them.

@@ -44,6 +44,8 @@ hipError_t launch_tree(const TreeArgs& a, int D, int is_f16, hipStream_t stream)
 
 // Keys per chunk and workgroup, from the sizes the host knows.
 int tree_chunk_keys(int B, int H, int T, int n_seg, const int64_t* scan);
+// Whether one workgroup takes all keys of a row and writes its outputs, without records and a merge.
+bool tree_whole_rows(int B, int H, int T, int n_seg, const int64_t* scan);
 
 struct CommitArgs {
   int B, H, T;
