@@ -2,7 +2,8 @@
  * sps_attn.h - C ABI of the MI355X (gfx950) SPS attention hot path.
  *
  * One shared library (libsps_attn.so) exports the three kernel families of the SPS Transformer's
- * attention path. All entry points are stateless, take plain device pointers, element strides and
+ * attention path, and attention with changed scores (caps, biases by distance, visible prefixes) in
+ * prefill, training and over drafted tokens. All entry points are stateless, take plain device pointers, element strides and
  * sizes, enqueue asynchronously on the caller's HIP stream (passed as void*, a hipStream_t), never
  * synchronise the host and never allocate device memory: scratch space is a caller-provided
  * workspace whose size the *_workspace_bytes functions report. They return SPS_OK or an error
@@ -36,6 +37,11 @@
  *                                    (attention/triton_sps_flash_attention.py:70-111); a
  *                                    verification entry point that materialises the mask the
  *                                    kernels evaluate.
+ * Without a counterpart there:
+ *   sps_biased_fwd / sps_biased_bwd  document-masked causal attention with capped and biased scores
+ *                                    and a visible prefix; the bias table's gradient
+ *   sps_tree_attention               drafted tokens (a tree, a chain, one token) over the KV segments
+ *   sps_commit_drafts                the accepted drafts appended to a cache
  */
 #ifndef SPS_ATTN_H
 #define SPS_ATTN_H
@@ -127,7 +133,8 @@ int sps_attn_bwd(int family, int B, int H, int N, int D, int dtype,
  * bucket(n), with e = num_buckets / 2 (rounded down) and M = max_distance: n for n < e, else
  * min(num_buckets - 1, e + floor((num_buckets - e) * log(n / e) / log(M / e))). 2 <= num_buckets <= 256,
  * e < M <= 512. Entries of the table below -16384 (-inf and the types' lowest values among them) hide
- * their pairs. softcap must be 0 or a positive finite number.
+ * their pairs. softcap must be 0 or in [2^-10, 2^20]; capped scores carry an absolute error of some
+ * 2^-22 softcap.
  */
 typedef struct sps_score_change {
   float softcap;
@@ -187,9 +194,10 @@ int sps_biased_bwd(int B, int H, int N, int D, int dtype,
  * Attention of T (1 .. 64) drafted tokens per sequence over up to 3 KV segments and the drafts' own
  * ancestors, with changed scores (`change` may be NULL: unchanged). q, draft_k, draft_v: [B, T, H, D] of
  * dtype (bf16 or f16, as the segments), strides {b, t, h}; segments as in sps_decode (strides {b, h, t},
- * t strides not negative). parents: [B, T] int32 or int64 (unit stride along T), or NULL for a chain: -1 (a child of the cached
- * sequence's last token) or the index of an earlier draft; a draft with any other value, or descending
- * from such a one, is no draft: it sees nothing, no draft sees it, and its output is 0. Positions for
+ * t strides not negative). parents: [B, T] int32 or int64 (unit stride along T), or NULL for a chain:
+ * -1 (a child of the cached sequence's last token) or the index of an earlier draft; a draft with any
+ * other value, or descending from such a one, is no draft: it sees nothing, no draft sees it, and its
+ * output is 0. Positions for
  * the distances run through the segments' live keys in their order; a draft's is their number plus its
  * depth. out: [B, T, H, D] of dtype, contiguous.
  * Workspace: sps_tree_workspace_bytes; a workspace of that size serves every call with the same D and T, no
@@ -212,10 +220,11 @@ int sps_tree_attention(int B, int H, int D, int T, int dtype,
 /*
  * Appends the accepted drafts of each sequence to its cache: the path from a root to draft last[b]
  * (parents as in sps_tree_attention; last: [B] int32 or int64) goes to rows len .. of k and v
- * [B, H, storage, D], and the length advances. Rows past the storage are dropped, and the length stops there; nothing happens where last[b]
- * is no draft or a length is negative or at the storage. Lengths: [B, H] (strides {b, h}) or, with
+ * [B, H, storage, D], and the length advances. Rows past the storage are dropped, and the length stops
+ * there; nothing happens where last[b] is no draft or a length is negative or at the storage. Lengths: [B, H] (strides {b, h}) or, with
  * len_per_head 0, [B]. dtype (bf16, f16 or fp32) is that of the cache and the drafts alike; strides are
- * {k: b, h, t, v: b, h, t} for the cache and {b, t, h} for the drafts. The caches may not overlap the drafts.
+ * {k: b, h, t, v: b, h, t} for the cache and {b, t, h} for the drafts. The drafts may not
+ * lie within the caches' memory, and no stride of the caches or lengths may be 0 (SPS_E_INVALID).
  */
 int sps_commit_drafts(int B, int H, int D, int T, int dtype,
                       void* k, void* v, const int64_t* kv_strides, int storage,

@@ -6,7 +6,7 @@
 //
 // Split over the keys: one workgroup per chunk of one segment and (sequence, head); the first chunk's also takes the
 // drafts among themselves. Each writes a partial record (accumulator, maximum, sum) per draft, and a second kernel
-// merges them. The pass is bound by HBM: every key and value is read once, 4 D bytes against 4 D T products, so at
+// merges them; a row of a single chunk goes straight to the outputs (tree_whole_rows). The pass is bound by HBM: every key and value is read once, 4 D bytes against 4 D T products, so at
 // T = 64 the matrix cores need a fifth of the time the bytes do. What counts is bytes in flight: a wave streams 32-key
 // blocks of its own through registers, loading ahead, passes each through LDS tiles of its own into the layouts of the
 // products, and meets the other waves only at the end. (Groups of blocks staged by direct global -> LDS loads with a
