@@ -1,9 +1,11 @@
 // C ABI of libsps_attn.so: argument validation, workspace layout and kernel dispatch.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <cstdlib>
 #include <cstring>
 #include <mutex>
 #include <string>
@@ -342,6 +344,9 @@ int check_change(const sps_score_change* c) {
   return SPS_OK;
 }
 
+// Workgroups of 512 threads, at most, whose threads a launch can count in 32 bits.
+constexpr int64_t kMaxGroups = (1 << 23) - 1;
+
 // Every product of the scale with the smallest cap's constants is finite.
 int check_scale(float sm_scale) {
   return std::fabs(sm_scale) <= 1e30f ? SPS_OK : fail(SPS_E_INVALID, "sm_scale must be finite and at most 1e30");
@@ -420,6 +425,8 @@ int sps_biased_fwd(int B, int H, int N, int D, int dtype, const void* q, const i
   if (rc || (rc = check_change(change)) || (rc = check_biased("prefix_len", prefix_len, prefix_dtype, D, dtype, sm_scale)))
     return rc;
   const int need = (int64_t)B * H * N > 0;
+  if ((int64_t)B * H * sps::q_tiles(N) > kMaxGroups)
+    return fail(SPS_E_UNSUPPORTED, "%lld workgroups: too many rows, heads or positions", (long long)B * H * sps::q_tiles(N));
   if ((rc = check_tensor("q", q, q_strides, need, N, D)) || (rc = check_tensor("k", k, k_strides, need, N, D)) ||
       (rc = check_tensor("v", v, v_strides, need, N, D)) || (rc = check_tensor("o", o, o_strides, need, N, D)))
     return rc;
@@ -457,6 +464,8 @@ int sps_biased_bwd(int B, int H, int N, int D, int dtype, const void* q, const i
   if (rc || (rc = check_change(change)) || (rc = check_biased("prefix_len", prefix_len, prefix_dtype, D, dtype, sm_scale)))
     return rc;
   const int need = (int64_t)B * H * N > 0;
+  if ((int64_t)B * H * sps::q_tiles(N) > kMaxGroups)
+    return fail(SPS_E_UNSUPPORTED, "%lld workgroups: too many rows, heads or positions", (long long)B * H * sps::q_tiles(N));
   if ((rc = check_tensor("q", q, q_strides, need, N, D)) || (rc = check_tensor("k", k, k_strides, need, N, D)) ||
       (rc = check_tensor("v", v, v_strides, need, N, D)) || (rc = check_tensor("o", o, o_strides, need, N, D)) ||
       (rc = check_tensor("dout", dout, dout_strides, need, N, D)) || (rc = check_tensor("dq", dq, dq_strides, need, N, D)) ||
@@ -608,6 +617,8 @@ int sps_tree_attention(int B, int H, int D, int T, int dtype, const void* q, con
   int chunk = sps::tree_chunk_keys(B, H, T, n_seg, seg_scan);
   while (workspace_bytes < tree_part_bytes(B, H, D, T, tree_chunks(n_seg, seg_scan, chunk)) && chunk < 4096) chunk *= 2;
   int64_t chunks = tree_chunks(n_seg, seg_scan, chunk);
+  if ((int64_t)B * H * std::max<int64_t>(chunks, T) > kMaxGroups)
+    return fail(SPS_E_UNSUPPORTED, "%lld workgroups: too many rows, chunks or drafts", (long long)B * H * std::max<int64_t>(chunks, T));
   const size_t need = tree_part_bytes(B, H, D, T, chunks);
   if (workspace_bytes < need) return fail(SPS_E_WORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, need);
   if (!workspace) return fail(SPS_E_INVALID, "workspace: null pointer");

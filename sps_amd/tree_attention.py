@@ -94,7 +94,8 @@ def tree_attention(
     ``parents_BxT``: [B, T] int32/int64, None for a chain (draft i follows draft i - 1). Segments, queries and drafts
     share one dtype; segments need not be contiguous. ``sm_scale``: 1 / sqrt(D) by default. ``softcap``, ``slopes``,
     ``bias_table``, ``max_distance``: as in ``biased_attention``; positions run through the segments' live keys in
-    their order, and a draft's position is their number plus its depth. Forward only (no gradients)."""
+    their order, and a draft's position is their number plus its depth. A draft's non-finite value row reaches every draft of
+    its sequence, whose weight of it may be 0; dead and padding rows reach none. Forward only (no gradients)."""
     if not torch.compiler.is_compiling():
         # Ordinary eager calls run in native code; None: the general path below.
         out = N.binding().tree_attention(q_BxTxHxD, segments, draft_k_BxTxHxD, draft_v_BxTxHxD, parents_BxT, sm_scale,

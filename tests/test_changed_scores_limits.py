@@ -55,3 +55,19 @@ def _commit(b=2, h=2, t=4, d=64, k=0x100000, v=0x200000, k_st=(8192, 4096, 64), 
 def test_commit_onto_shared_memory(over, needle):
     assert _commit(**over) == N.SPS_E_INVALID and needle in N.last_error()
 
+
+
+@cpu_only
+def test_more_workgroups_than_a_launch_has():
+    st, change = N.i64_array((0, 0, 64)), N.ScoreChange(softcap=1.0)
+    assert N.lib().sps_biased_fwd(4096, 4096, 128, 64, N.DTYPE_BF16, *(0x10000, st) * 4, 0x20000, None, 0, 0, None, N.DTYPE_I32,
+                                  1.0, C.byref(change), None, 0, None) == N.SPS_E_UNSUPPORTED
+    assert "workgroups" in N.last_error()
+    ds = N.i64_array((512, 128, 64))
+    scan = N.i64_array([100])
+    rows = N.i64_array((0, 0, 64))
+    ptr, one = N.ptr_const((0x10000,)), N.i32_const((1,))
+    assert N.lib().sps_tree_attention(4096, 4096, 64, 1, N.DTYPE_BF16, 0x10000, ds, 1, ptr, rows, ptr, rows, ptr,
+                                      N.i32_const((N.DTYPE_I64,)), one, scan, 0x10000, ds, 0x10000, ds, None, N.DTYPE_I32, 1,
+                                      1.0, None, 0x20000, 0x30000, 1 << 40, None) == N.SPS_E_UNSUPPORTED
+    assert "workgroups" in N.last_error()
